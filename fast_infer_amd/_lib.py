@@ -71,6 +71,19 @@ SIGNATURES = {
          _f32,                                   # sm_scale
          _ptr],                                  # stream
     ),
+    "fi_paged_chunk_attention_workspace_size": (_sz, [_i64, _i64, _i64, _i64, _i64, _i64]),
+    "fi_paged_chunk_attention_fwd": (
+        ctypes.c_int,
+        [_ptr, _i64, _i64, _i64,                 # q, strides
+         _ptr, _ptr, _i64, _i64, _i64,           # pools, N, block_size, Hkv
+         _ptr, _i64, _i64,                       # block table, stride, max blocks
+         _ptr, _ptr, _i64,                       # start_positions, context_lens, num_tokens
+         _ptr, _i64, _i64, _i64,                 # o, strides
+         _i64, _i64, _i64, _i64,                 # batch, new tokens, Hq, D
+         _f32, _f32, _ptr, _i64, _ptr,           # sm_scale, softcap, slopes, window, prefix_lens
+         _ptr, _sz,                              # workspace
+         _ptr],                                  # stream
+    ),
     "fi_kv_store": (
         ctypes.c_int,
         [_ptr, _i64, _i64, _i64,
@@ -128,6 +141,13 @@ SIGNATURES = {
         ctypes.c_int, [_ptr, _i64, _ptr, _i64, _i64, _i64, _i64, _ptr, _i64, _ptr],
     ),
     "fi_rmsnorm": (ctypes.c_int, [_ptr, _i64, _i64, _i64, _ptr, _f32, _ptr, _i64, _ptr]),
+    "fi_add_rmsnorm": (
+        ctypes.c_int,
+        [_ptr, _i64, _ptr, _i64, _i64, _i64,     # x, residual, strides, M, hidden
+         _ptr, _f32,                             # weight, eps
+         _ptr, _i64, _ptr, _i64,                 # h_out, out, strides
+         _ptr],                                  # stream
+    ),
     "fi_rmsnorm_int4_matmul_workspace_size": (_sz, [_i64, _i64, _i64]),
     "fi_rmsnorm_int4_matmul": (
         ctypes.c_int,
@@ -153,6 +173,8 @@ FI_KV_NEGATIVE_COUNT = 3
 # entry points the wrappers call once per launch
 FAST = ("fi_flash_attention_fwd", "fi_paged_attention_fwd", "fi_rope_store_kv", "fi_int4_matmul",
         "fi_rmsnorm", "fi_rmsnorm_int4_matmul")
+# the same, of steps that continue cached sequences
+FAST_CHUNK = ("fi_paged_chunk_attention_fwd", "fi_add_rmsnorm")
 
 _lib = None
 _calls = None
@@ -185,7 +207,7 @@ def load() -> ctypes.CDLL:
         except ImportError:  # not built (no compiler or headers for it): the same calls, slower
             _calls = lib
         else:
-            for name in FAST:
+            for name in FAST + FAST_CHUNK:
                 _fastcall.bind(name, ctypes.cast(getattr(lib, name), ctypes.c_void_p).value)
             _calls = _fastcall
         _lib = lib
@@ -193,7 +215,7 @@ def load() -> ctypes.CDLL:
 
 
 def calls():
-    """The entry points of ``FAST`` as native functions (csrc/fastcall.c): positional integers
+    """The entry points of ``FAST`` and ``FAST_CHUNK`` as native functions (csrc/fastcall.c): positional integers
     (None for a null pointer) and floats, the return code back.  The wrappers' call path; every
     other use goes through ``load()``, as the wrappers' calls do where that module is not built."""
     if _calls is None:

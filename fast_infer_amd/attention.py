@@ -15,6 +15,10 @@ reference behaviour:
 * ``paged_attention(..., context_lens=)`` — per-row context lengths (the reference
   has one shared ``num_tokens``); ``num_tokens`` may also be given as an int32
   tensor of per-row lengths.
+
+``paged_chunk_attention`` has no counterpart in the reference: several new tokens per
+sequence attend over the paged pool, with optional capped scores, distance bias, sliding
+window and prefix mask (single tokens of models that need those included).
 """
 
 from __future__ import annotations
@@ -240,6 +244,132 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         ws_ptr, ws_bytes,
         _lib.tensor_stream(q))
     _lib.check(rc, "paged_attention")
+    if work is not o:
+        o.copy_(work)
+    return o
+
+
+def paged_chunk_attention_workspace(batch: int, num_new: int, num_q_heads: int, num_kv_heads: int,
+                                    num_tokens: int, head_dim: int, device) -> torch.Tensor | None:
+    """Device scratch for the partial results of one paged_chunk_attention call (or None)."""
+    nbytes = _lib.load().fi_paged_chunk_attention_workspace_size(
+        batch, num_new, num_q_heads, num_kv_heads, num_tokens, head_dim)
+    if nbytes == 0:
+        return None
+    return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
+def _per_row(name: str, t: torch.Tensor, batch: int, dev: int) -> torch.Tensor:
+    """A per-row int32 tensor on device index `dev`, contiguous, with at least `batch` entries."""
+    if t.dtype is not torch.int32 or t.get_device() != dev:
+        t = t.to(device=torch.device("cuda", dev), dtype=torch.int32)
+    if t.numel() < batch:
+        raise ValueError(f"{name} has fewer entries than the batch")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                          block_table: torch.Tensor, block_size: int, num_tokens,
+                          sm_scale: float = None, *,
+                          start_positions: torch.Tensor | None = None,
+                          context_lens: torch.Tensor | None = None,
+                          softcap: float | None = None,
+                          alibi_slopes: torch.Tensor | None = None,
+                          window: int | None = None,
+                          prefix_lens: torch.Tensor | None = None,
+                          workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a chunk of new tokens over the paged pool, which already holds their K/V.
+
+    q: [batch, num_new, num_q_heads, head_dim] fp16; pools, ``block_table``, ``num_tokens``
+    and ``context_lens`` as in ``paged_attention`` (lengths count the new tokens).  Token t of
+    row b stands at position ``start_positions[b] + t``; without ``start_positions`` the chunk
+    is the row's last ``num_new`` tokens.  ``PagedKVCache.append`` returns both tensors.  A token
+    sees the keys up to its own position; tokens at or past the row's length (padding) and
+    tokens that see no key give zeros.  Options:
+
+    * ``softcap``: scores become ``softcap * tanh(s / softcap)``, s scaled by ``sm_scale``;
+    * ``alibi_slopes`` fp32 ``[num_q_heads]``: ``slope * |position - key|`` is subtracted;
+    * ``window``: a token sees the last ``window`` positions up to its own only;
+    * ``prefix_lens`` int32 ``[batch]``: positions every token of the row sees, those behind it
+      and outside the window included.
+
+    ``workspace`` (``paged_chunk_attention_workspace``) must not be shared by calls that
+    overlap in time; by default one is allocated per call.  Returns o with q's shape and
+    strides."""
+    batch, num_new, num_q_heads, head_dim = q.shape
+    if sm_scale is None:
+        sm_scale = head_dim ** -0.5
+    _check_fp16_cuda("q", q)
+    _check_fp16_cuda("k_cache", k_cache)
+    _check_fp16_cuda("v_cache", v_cache)
+    dev = q.get_device()
+    if k_cache.get_device() != dev or v_cache.get_device() != dev:
+        raise RuntimeError("the pools must be on the same device as q")
+    pool_shape = k_cache.shape
+    if len(pool_shape) != 4 or v_cache.shape != pool_shape:
+        raise ValueError("k_cache/v_cache must be [num_blocks, block_size, kv_heads, dim]")
+    num_blocks, pool_bs, num_kv_heads, pool_dim = pool_shape
+    if pool_bs != block_size or pool_dim != head_dim:
+        raise ValueError(f"pool shape {tuple(pool_shape)} does not match block_size "
+                         f"{block_size} / head_dim {head_dim}")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous()):
+        raise ValueError("pools must be contiguous")
+    if num_kv_heads == 0 or num_q_heads % num_kv_heads:
+        raise ValueError(f"num_q_heads {num_q_heads} not a multiple of kv heads {num_kv_heads}")
+    block_table = _check_table(block_table, dev)
+    bt_rows, bt_cols = block_table.shape
+    if bt_rows < batch:
+        raise ValueError("block_table has fewer rows than the batch")
+    if isinstance(num_tokens, torch.Tensor):
+        if context_lens is not None:
+            raise ValueError("give per-row lengths either as num_tokens or as context_lens")
+        context_lens = num_tokens
+        num_tokens = bt_cols * block_size
+    num_tokens = int(num_tokens)
+    if context_lens is not None:
+        context_lens = _per_row("context_lens", context_lens, batch, dev)
+    if start_positions is not None:
+        start_positions = _per_row("start_positions", start_positions, batch, dev)
+    if prefix_lens is not None:
+        prefix_lens = _per_row("prefix_lens", prefix_lens, batch, dev)
+    if softcap is not None and not softcap > 0:
+        raise ValueError(f"softcap must be positive, got {softcap}")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if alibi_slopes is not None:
+        if alibi_slopes.shape != (num_q_heads,):
+            raise ValueError(f"alibi_slopes must be [{num_q_heads}], got {tuple(alibi_slopes.shape)}")
+        if alibi_slopes.dtype is not torch.float32 or alibi_slopes.get_device() != dev:
+            alibi_slopes = alibi_slopes.to(device=q.device, dtype=torch.float32)
+        if not alibi_slopes.is_contiguous():
+            alibi_slopes = alibi_slopes.contiguous()
+    o = torch.empty_like(q)
+    if batch == 0 or num_new == 0 or num_q_heads == 0:
+        return o
+    q, qs, q_ptr = _prep_rows(q)
+    os_, o_ptr = o.stride(), o.data_ptr()
+    if _strides_ok(os_, o_ptr):
+        work = o
+    else:
+        work = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        os_, o_ptr = work.stride(), work.data_ptr()
+    need = _lib.workspace_size("fi_paged_chunk_attention_workspace_size", batch, num_new,
+                               num_q_heads, num_kv_heads, num_tokens, head_dim)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ws_ptr = workspace.data_ptr() if need else None
+    ws_bytes = workspace.numel() * workspace.element_size() if need else 0
+    rc = _lib.calls().fi_paged_chunk_attention_fwd(
+        q_ptr, qs[0], qs[1], qs[2],
+        k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, block_size, num_kv_heads,
+        block_table.data_ptr(), block_table.stride(0), bt_cols,
+        _ptr(start_positions), _ptr(context_lens), num_tokens,
+        o_ptr, os_[0], os_[1], os_[2],
+        batch, num_new, num_q_heads, head_dim,
+        float(sm_scale), float(softcap or 0.0), _ptr(alibi_slopes), int(window or 0),
+        _ptr(prefix_lens), ws_ptr, ws_bytes,
+        _lib.tensor_stream(q))
+    _lib.check(rc, "paged_chunk_attention")
     if work is not o:
         o.copy_(work)
     return o

@@ -42,6 +42,8 @@ HIPCC_FLAGS = [
 # -inf (not NaN), so its max operations need no NaN quieting (saves a v_max per input).
 FILE_FLAGS = {
     "flash_prefill.hip": ["-fno-honor-nans"],
+    # the same; where it looks for NaN (masked keys), it compares bits
+    "paged_chunk.hip": ["-fno-honor-nans"],
 }
 
 

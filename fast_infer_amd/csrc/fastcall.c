@@ -13,7 +13,7 @@
 #include "../../include/fast_infer_amd.h"
 
 // One argument list by its format: 'p' pointer (an integer address or None), 'i' integer, 'f'
-// float.  Integers go to v in order, the float to *f.  0, or -1 with an exception set.
+// float.  Integers go to v in order, floats to f.  0, or -1 with an exception set.
 static int parse(const char* name, const char* fmt, PyObject* const* args, Py_ssize_t n, int64_t* v,
                  float* f) {
   if ((size_t)n != strlen(fmt)) {
@@ -25,7 +25,7 @@ static int parse(const char* name, const char* fmt, PyObject* const* args, Py_ss
     if (fmt[i] == 'f') {
       const double d = PyFloat_AsDouble(a);
       if (d == -1.0 && PyErr_Occurred()) return -1;
-      *f = (float)d;
+      *f++ = (float)d;
     } else if (fmt[i] == 'p' && a == Py_None) {
       *v++ = 0;
     } else {
@@ -38,19 +38,21 @@ static int parse(const char* name, const char* fmt, PyObject* const* args, Py_ss
 }
 
 #define MAX_ARGS 40
+#define MAX_FLOATS 2
 #define CALL(name, fmt, ...)                                                            \
   static __typeof__(&name) name##_fn;                                                   \
   static PyObject* py_##name(PyObject* self, PyObject* const* args, Py_ssize_t n) {     \
     (void)self;                                                                         \
     _Static_assert(sizeof(fmt) <= MAX_ARGS + 1, "argument buffer");                      \
     int64_t v[MAX_ARGS];                                                                \
-    float f = 0.f;                                                                      \
+    float fs[MAX_FLOATS] = {0.f};                                                       \
     int rc;                                                                             \
     if (!name##_fn) {                                                                   \
       PyErr_SetString(PyExc_RuntimeError, #name " is not bound");                       \
       return NULL;                                                                      \
     }                                                                                   \
-    if (parse(#name, fmt, args, n, v, &f)) return NULL;                                 \
+    if (parse(#name, fmt, args, n, v, fs)) return NULL;                                 \
+    const float f = fs[0];                                                              \
     (void)f;                                                                            \
     Py_BEGIN_ALLOW_THREADS rc = name##_fn(__VA_ARGS__);                                 \
     Py_END_ALLOW_THREADS return PyLong_FromLong(rc);                                    \
@@ -67,6 +69,12 @@ CALL(fi_paged_attention_fwd, "piippiiipiipipiiiiifpip",
        v[7], (const int32_t*)v[8], v[9], v[10], (const int32_t*)v[11], v[12], (void*)v[13],
        v[14], v[15], v[16], v[17], v[18], f, (void*)v[19], (size_t)v[20], (void*)v[21])
 
+CALL(fi_paged_chunk_attention_fwd, "piiippiiipiippipiiiiiiiffpippip",
+       (const void*)v[0], v[1], v[2], v[3], (const void*)v[4], (const void*)v[5], v[6], v[7],
+       v[8], (const int32_t*)v[9], v[10], v[11], (const int32_t*)v[12], (const int32_t*)v[13],
+       v[14], (void*)v[15], v[16], v[17], v[18], v[19], v[20], v[21], v[22], f, fs[1], (const
+       float*)v[23], v[24], (const int32_t*)v[25], (void*)v[26], (size_t)v[27], (void*)v[28])
+
 CALL(fi_rope_store_kv, "piiipiiipiiippipiiipiiippiipiiiiiiiipp",
        (const void*)v[0], v[1], v[2], v[3], (const void*)v[4], v[5], v[6], v[7], (const
        void*)v[8], v[9], v[10], v[11], (const void*)v[12], (const void*)v[13], v[14],
@@ -82,6 +90,10 @@ CALL(fi_rmsnorm, "piiipfpip",
        (const void*)v[0], v[1], v[2], v[3], (const void*)v[4], f, (void*)v[5], v[6],
        (void*)v[7])
 
+CALL(fi_add_rmsnorm, "pipiiipfpipip",
+       (const void*)v[0], v[1], (const void*)v[2], v[3], v[4], v[5], (const void*)v[6], f,
+       (void*)v[7], v[8], (void*)v[9], v[10], (void*)v[11])
+
 CALL(fi_rmsnorm_int4_matmul, "piiipfpipiiipipip",
        (const void*)v[0], v[1], v[2], v[3], (const void*)v[4], f, (const void*)v[5], v[6],
        (const void*)v[7], v[8], v[9], v[10], (void*)v[11], v[12], (void*)v[13],
@@ -90,9 +102,11 @@ CALL(fi_rmsnorm_int4_matmul, "piiipfpipiiipipip",
 #define NAMES(X)           \
   X(fi_flash_attention_fwd) \
   X(fi_paged_attention_fwd) \
+  X(fi_paged_chunk_attention_fwd) \
   X(fi_rope_store_kv) \
   X(fi_int4_matmul) \
   X(fi_rmsnorm) \
+  X(fi_add_rmsnorm) \
   X(fi_rmsnorm_int4_matmul)
 
 // bind(name, address): the entry point `name` of the loaded library.

@@ -1,0 +1,800 @@
+// Attention of a chunk of new tokens over a paged KV pool [num_blocks, block_size,
+// num_kv_heads, head_dim], for gfx950: the form between causal prefill (no cache) and decode
+// (one token): prompts prefilled in pieces or behind a cached beginning, drafted tokens, single
+// tokens of models whose scores are capped, biased or windowed.
+//
+//   x[t, j] = sm_scale * q[t] . k[j]            position pos = start + t, key j < len
+//   x       = cap * tanh(x / cap)               (with a cap)
+//   x      -= slope[h] * |pos - j|              (with a distance bias)
+//   o[t]    = sum_j softmax_j(x[t, j]) v[j]     over the keys token t sees:
+//             j < prefix, or pos - window < j <= pos
+//
+// Layout for MI355X:
+//   * The query rows of one kv head are the pairs (token, head of the group), token-major, and a
+//     workgroup takes 64 * NB consecutive ones, whatever the group size: 16 * NB per wave, one
+//     row per MFMA column.  Each 64-key K/V tile staged in LDS serves all of them.
+//   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: the lane that holds a query
+//     column keeps its scores, P and O; the softmax (online, fp32, base 2) needs no shuffles.
+//   * Tiles are copied global -> LDS without registers, two stages.  Every lane carries the
+//     64-bit address of its own piece of a key's row, looked up in the block table one tile
+//     ahead, so that any block size and any pool size take the same path; keys at or past the
+//     row's length, or behind an invalid table entry, are read from a page of zeros.
+//   * Few query rows: the row tile's list of key tiles is cut into parts, by its own true
+//     length, on the device; the parts' unnormalised results are added by a second kernel.
+#include <algorithm>
+#include <cmath>
+
+#include "common.h"
+
+namespace fi {
+namespace chunk {
+
+constexpr int kWaves = 4;
+constexpr int kThreads = kWaves * 64;
+constexpr int kKTile = 64;                      // keys per tile
+constexpr int kRowBytes = kHeadDim * 2;         // one K or V row in LDS
+constexpr int kTileBytes = kKTile * kRowBytes;  // 16 KiB
+constexpr int kStageBytes = 2 * kTileBytes;     // K + V
+constexpr int kMaxNb = 3;
+constexpr float kLazyLog2 = 8.f;  // the reference max may lag the true max by 2^8
+constexpr int kNoWindow = 0x3fffffff;
+constexpr int64_t kMaxTokens = (int64_t)1 << 22;
+// Largest cap whose tanh is taken from exp2 alone: its absolute error, about 2e-7, times the
+// cap is an error of the logit, here 1e-4.
+constexpr float kExpCap = 500.f;
+
+constexpr int kCap = 1;   // kMod bits: capped scores,
+constexpr int kBias = 2;  // distance bias
+
+// n / d for 0 <= n < 2^31 by a multiplication.
+struct FastDiv {
+  uint32_t mul;
+  int shift;
+};
+static FastDiv fast_div(uint32_t d) {
+  int l = 0;
+  while (((uint64_t)1 << l) < d) ++l;
+  return {(uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << l) - d)) / d + 1), l};
+}
+__device__ __forceinline__ int div_by(int n, FastDiv d) {
+  return (int)((__umulhi((uint32_t)n, d.mul) + (uint32_t)n) >> d.shift);
+}
+
+struct Params {
+  const half_t* q;
+  int64_t q_sb, q_st, q_sh;
+  const half_t* k_cache;
+  const half_t* v_cache;
+  int num_pool_blocks;
+  int block_size;
+  FastDiv block_div;
+  int num_kv_heads;
+  int64_t row_bytes;  // one pool slot, all kv heads
+  const int32_t* block_table;
+  int64_t bt_stride;
+  int max_blocks_per_seq;
+  const int32_t* start_positions;
+  const int32_t* context_lens;
+  int num_tokens;  // bound of the lengths, at most the table's width
+  half_t* o;
+  int64_t o_sb, o_st, o_sh;
+  int batch, chunk;
+  int num_q_heads;
+  int group;
+  FastDiv group_div;
+  int head_dim;
+  int d_chunks;       // 16-byte chunks of a row; those past it are read as zeros
+  float scale_log2;   // score unit -> log2 unit (1 with a cap: those scores are made in log2 units)
+  float lazy_raw;     // kLazyLog2 in score units
+  float lazy_log2;    // lazy_raw * scale_log2
+  uint32_t q_sign;    // 0x80008000: Q negated (negative sm_scale without a cap)
+  int q_zero;         // sm_scale == 0 without a cap: Q read as zeros
+  float cap_arg;      // sm_scale / cap
+  float cap_log2;     // cap * log2(e)
+  const float* slopes;
+  float slope_mul;    // slope unit -> score unit
+  int window;
+  const int32_t* prefix_lens;
+  int rows_per_tile;  // 64 * NB
+  int max_splits;
+  int min_part;       // key tiles of the smallest part
+  float* part_o;      // [batch * chunk * num_q_heads][max_splits][128]; null: write o
+  float* part_ml;     // [...][2]: reference max (log2 units), sum
+};
+
+// What a batch row attends over.
+struct Row {
+  int start, len, prefix;
+};
+__device__ __forceinline__ Row row_of(const Params& p, int b) {
+  Row r;
+  int len = p.context_lens ? p.context_lens[b] : p.num_tokens;
+  len = min(len, p.num_tokens);
+  r.len = max(len, 0);
+  int s = p.start_positions ? p.start_positions[b] : r.len - p.chunk;
+  r.start = max(min(s, r.len), -p.chunk);
+  int pre = p.prefix_lens ? p.prefix_lens[b] : 0;
+  r.prefix = max(min(pre, r.len), 0);
+  return r;
+}
+
+// Positions of the valid tokens among query rows r0 .. r1 (lo > hi: none).
+__device__ __forceinline__ void row_positions(const Params& p, const Row& row, int r0, int r1, int& lo,
+                                              int& hi) {
+  lo = max(row.start + div_by(r0, p.group_div), 0);
+  hi = min(row.start + min(div_by(r1, p.group_div), p.chunk - 1), row.len - 1);
+}
+
+// The key tiles a row tile visits: tiles 0 .. n_pre - 1 (prefix), then from `from` on.
+struct Span {
+  int n_pre, from, n;
+  __device__ __forceinline__ int tile(int i) const { return i < n_pre ? i : from + i - n_pre; }
+};
+__device__ __forceinline__ Span span_of(const Params& p, const Row& row, int lo, int hi) {
+  Span s;
+  s.n_pre = (row.prefix + kKTile - 1) / kKTile;
+  s.from = max(max(lo - p.window + 1, 0) / kKTile, s.n_pre);
+  s.n = s.n_pre + max((hi + kKTile) / kKTile - s.from, 0);
+  if (lo > hi) s.n = 0;
+  return s;
+}
+__device__ __forceinline__ int part_size(const Params& p, int n) {
+  return max((n + p.max_splits - 1) / p.max_splits, p.min_part);
+}
+
+// LDS tile layouts, as in the prefill kernel: a K tile is 4 panels of 64 bytes per key (chunks
+// XOR-permuted by (key >> 1) & 3, conflict-free fragment reads), a V tile 8 panels of 32 bytes
+// per key (conflict-free transpose reads).
+constexpr int kKPanel = kKTile * 64;
+constexpr int kVPanel = kKTile * 32;
+
+// The page that masked keys and the columns past head_dim are copied from.
+__device__ __attribute__((aligned(256))) const char g_zeros[kRowBytes] = {0};
+
+// One direct-to-LDS copy from a 64-bit address per lane: 16 bytes to LDS byte lds + 16 * lane.
+// Through inline asm for the reasons given at lds_copy16; the callers wait for the copies
+// themselves.  M0 takes one idle slot before a global load reads it.
+__device__ __forceinline__ void lds_copy16_global(const char* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(src)
+               : "memory");
+}
+
+// This wave's copies have landed, its LDS reads are done, and every other wave says the same.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// This wave's eight copies (four of K, four of V) of the tile whose key `lane` lies in pool row
+// `row` (-1: zeros).  Wave w copies K keys 16w .. 16w + 15 and half the columns of V keys
+// 32 (w / 2) .. + 31.
+__device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, const char* vbase,
+                                           char* stage, int row, int w, int lane) {
+  const int rk = __shfl(row, 16 * w + (lane >> 2));
+  const int rv = __shfl(row, 32 * (w >> 1) + (lane >> 1));
+  const char* ks = rk >= 0 ? kbase + rk * p.row_bytes : g_zeros;
+  const char* vs = rv >= 0 ? vbase + rv * p.row_bytes : g_zeros;
+  const uint32_t kd = lds_addr(stage) + 16 * w * 64;
+  const uint32_t vd = lds_addr(stage) + kTileBytes + 32 * (w >> 1) * 32;
+  const int kc = (lane & 3) ^ ((lane >> 3) & 3);
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int ch = 4 * q + kc;
+    lds_copy16_global(ch < p.d_chunks ? ks + 16 * ch : g_zeros, kd + q * kKPanel);
+    const int panel = 4 * (w & 1) + q;
+    const int vch = 2 * panel + (lane & 1);
+    lds_copy16_global(vch < p.d_chunks ? vs + 16 * vch : g_zeros, vd + panel * kVPanel);
+  }
+}
+
+// V^T fragment half: lane (col, g) receives keys row0 + 4g + j (j = 0..3) of column 16 dt + col.
+__device__ __forceinline__ u32x2 vt_read(const char* vs, int row0, int dt, int col, int g) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  const char* ptr = vs + dt * kVPanel + (row0 + 4 * g + (col >> 2)) * 32 + ((col & 3) << 3);
+  const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3)))*)ptr);
+  return __builtin_bit_cast(u32x2, v);
+}
+__device__ __forceinline__ half8 vt_frag(const char* vs, int c, int dt, int col, int g) {
+  const u32x2 a0 = vt_read(vs, 32 * c, dt, col, g);
+  const u32x2 a1 = vt_read(vs, 32 * c + 16, dt, col, g);
+  return as_half8(u32x4{a0[0], a0[1], a1[0], a1[1]});
+}
+
+// S^T = K Q^T + init for the 32-key slice c: s[j][t] holds keys 32c + 16t + 4g + r of row block j.
+template <int NB>
+__device__ __forceinline__ void qk_slice(const char* ks, int c, int col, int g,
+                                         const half8 (&qf)[NB][4], floatx4 (&s)[NB][2]) {
+  auto frag = [&](int u) {
+    const int t = u >> 2, i = u & 3;
+    return as_half8(*(const u32x4*)(ks + i * kKPanel + (32 * c + 16 * t + col) * 64 +
+                                    ((g ^ ((col >> 1) & 3)) << 4)));
+  };
+  half8 cur = frag(0);
+#pragma unroll
+  for (int u = 0; u < 8; ++u) {
+    half8 nxt;
+    if (u + 1 < 8) nxt = frag(u + 1);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) s[j][u >> 2] = mfma16x16x32(cur, qf[j][u & 3], s[j][u >> 2]);
+    if (u + 1 < 8) cur = nxt;
+  }
+}
+
+// O^T += V^T P^T of slice c (accumulator tiles 0..7) and the sums of P (tile 8, all-ones A).
+template <int NB>
+__device__ __forceinline__ void pv_slice(const char* vs, int c, int col, int g, const half8 (&pf)[NB],
+                                         floatx4 (&acc)[NB][9]) {
+  half8 vf = vt_frag(vs, c, 0, col, g);
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) {
+    half8 vn;
+    if (dt + 1 < 8) vn = vt_frag(vs, c, dt + 1, col, g);
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[j][dt] = mfma16x16x32(vf, pf[j], acc[j][dt]);
+    if (dt + 1 < 8) vf = vn;
+  }
+  const half8 ones = as_half8(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
+#pragma unroll
+  for (int j = 0; j < NB; ++j) acc[j][8] = mfma16x16x32(ones, pf[j], acc[j][8]);
+}
+
+// Whether slice c of V is finite: the product with an all-zero P is NaN where V is not.
+__device__ __forceinline__ bool v_finite(const char* vs, int c, int col, int g) {
+  const half8 zero = as_half8(u32x4{0u, 0u, 0u, 0u});
+  floatx4 chk = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) chk = mfma16x16x32(vt_frag(vs, c, dt, col, g), zero, chk);
+  // the file is compiled for NaN-free arithmetic: hide where the bits are from
+  asm volatile("" : "+v"(chk));
+  const u32x4 u = __builtin_bit_cast(u32x4, chk);
+  const uint32_t bad = (u[0] | u[1] | u[2] | u[3]) & 0x7fffffffu;
+  return __builtin_amdgcn_ballot_w64(bad != 0) == 0;
+}
+
+// pv_slice where a key that some rows must not see may hold an infinity or a NaN in V: 0 * inf
+// in the matrix product would reach those rows.  The product runs on V with such values
+// replaced by zeros; then products of indicators (V is +inf or NaN / -inf or NaN; P is not zero)
+// count which of them each row sees, and put the infinities where they belong (both: NaN).
+template <int NB>
+__device__ __forceinline__ void pv_slice_careful(const char* vs, int c, int col, int g,
+                                                 const half8 (&pf)[NB], floatx4 (&acc)[NB][9]) {
+  typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+  for (int dt = 0; dt < 8; ++dt) {
+    const us8 v = __builtin_bit_cast(us8, vt_frag(vs, c, dt, col, g));
+    us8 ok, inf[2];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned short m = v[e] & 0x7fff;
+      ok[e] = m < 0x7c00 ? v[e] : (unsigned short)0;
+      inf[0][e] = m > 0x7c00 || v[e] == 0x7c00 ? (unsigned short)0x3c00 : (unsigned short)0;
+      inf[1][e] = m > 0x7c00 || v[e] == 0xfc00 ? (unsigned short)0x3c00 : (unsigned short)0;
+    }
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      acc[j][dt] = mfma16x16x32(__builtin_bit_cast(half8, ok), pf[j], acc[j][dt]);
+      us8 pi = __builtin_bit_cast(us8, pf[j]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pi[e] = pi[e] ? (unsigned short)0x3c00 : (unsigned short)0;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const floatx4 n = mfma16x16x32(__builtin_bit_cast(half8, inf[i]), __builtin_bit_cast(half8, pi),
+                                       floatx4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = n[r] > 0.f ? (i ? -__builtin_inff() : __builtin_inff()) : 0.f;
+          asm volatile("" : "+v"(x));  // the sum of both infinities has to be taken, not folded
+          acc[j][dt][r] += x;
+        }
+      }
+    }
+  }
+  const half8 ones = as_half8(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
+#pragma unroll
+  for (int j = 0; j < NB; ++j) acc[j][8] = mfma16x16x32(ones, pf[j], acc[j][8]);
+}
+
+// x = cap_log2 * tanh(s * cap_arg), in log2 units.  tanh(y) = 1 - 2 / (1 + e^2y); for large caps,
+// where its absolute error would show, its series below 1/4 (the next term is under 2e-8).
+__device__ __forceinline__ float capped(const Params& p, float s, bool series) {
+  const float y = s * p.cap_arg;
+  const float e = fast_exp2(y * (2.f * kLog2e));
+  float x = __builtin_fmaf(-2.f * p.cap_log2, __builtin_amdgcn_rcpf(1.f + e), p.cap_log2);
+  if (series) {
+    const float z = y * y;
+    float t = __builtin_fmaf(z, 62.f / 2835.f, -17.f / 315.f);
+    t = __builtin_fmaf(z, t, 2.f / 15.f);
+    t = __builtin_fmaf(z, t, -1.f / 3.f);
+    t = __builtin_fmaf(z * y, t, y);
+    if (__builtin_fabsf(y) < 0.25f) x = p.cap_log2 * t;
+  }
+  return x;
+}
+
+// One resident tile (keys k0 .. k0 + 63) for this wave's rows.  s_pos: positions of the
+// workgroup's rows; keys: bit k is set when key k0 + k is before the row's length and in the
+// pool; masked: some row does not see some key.
+template <int NB, int kMod>
+__device__ __forceinline__ void consume(const Params& p, const char* stage, int k0, uint64_t keys,
+                                        bool masked, int prefix, const int* s_pos,
+                                        const float* s_slope, int col, int g,
+                                        const half8 (&qf)[NB][4], float (&t_run)[NB],
+                                        floatx4 (&acc)[NB][9]) {
+  const char* ks = stage;
+  const char* vs = stage + kTileBytes;
+#pragma unroll
+  for (int c = 0; c < kKTile / 32; ++c) {
+    // a uniform branch, never taken, between the slices: without it the compiler overlaps the
+    // unrolled slices beyond the register file
+    if (p.chunk < 0) break;
+    const int key0 = k0 + 32 * c + 4 * g;  // lane's key of (t, r): key0 + 16t + r
+    floatx4 s[NB][2];
+    auto bias = [&](int j, int t, int r) {
+      return -s_slope[16 * j + col] * __builtin_fabsf((float)(s_pos[16 * j + col] - key0 - 16 * t - r));
+    };
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[j][t][r] = kMod == kBias ? bias(j, t, r) : 0.f;
+    qk_slice<NB>(ks, c, col, g, qf, s);
+    if (kMod & kCap) {
+      const bool series = p.cap_log2 > kExpCap * kLog2e;
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            s[j][t][r] = capped(p, s[j][t][r], series);
+            if (kMod & kBias) s[j][t][r] += bias(j, t, r);
+          }
+    }
+    if (masked) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const int pos = s_pos[16 * j + col];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int key = key0 + 16 * t + r;
+            const bool see = (key < prefix || (key <= pos && key > pos - p.window)) &&
+                             ((keys >> (key - k0)) & 1);
+            if (!see) s[j][t][r] = -__builtin_inff();
+          }
+      }
+    }
+    // Online softmax with a lazily moved reference max, kept as the threshold t = max + slack in
+    // score units: it moves only when a score exceeds it (p <= 2^8, exact in fp16; sums in fp32).
+    bool move = false;
+    float lmax[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const float x = fmaxf(fmaxf(s[j][0][0], s[j][0][1]), fmaxf(s[j][0][2], s[j][0][3]));
+      lmax[j] = fmaxf(fmaxf(fmaxf(s[j][1][0], s[j][1][1]), fmaxf(s[j][1][2], s[j][1][3])), x);
+      move |= lmax[j] > t_run[j];
+    }
+    if (__builtin_amdgcn_ballot_w64(move)) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        const float t_old = t_run[j];
+        const float rmax = row4_max(lmax[j]);
+        const float t_new = rmax > t_old ? rmax + p.lazy_raw : t_old;
+        const float alpha = fast_exp2((t_old - t_new) * p.scale_log2);
+        t_run[j] = t_new;
+#pragma unroll
+        for (int dt = 0; dt < 9; ++dt) acc[j][dt] *= alpha;
+      }
+    }
+    // P is rounded to fp16 for the matrix cores; the sums take the rounded values too.
+    half8 pf[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const float mc = __builtin_fmaf(t_run[j], p.scale_log2, -p.lazy_log2);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          pf[j][4 * t + r] = (half_t)fast_exp2(__builtin_fmaf(s[j][t][r], p.scale_log2, -mc));
+    }
+    if (masked && !v_finite(vs, c, col, g))
+      pv_slice_careful<NB>(vs, c, col, g, pf, acc);
+    else
+      pv_slice<NB>(vs, c, col, g, pf, acc);
+  }
+}
+
+template <int NB, int kMod>
+__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
+  constexpr int kRowsPerWave = 16 * NB;
+  constexpr int kRows = kWaves * kRowsPerWave;
+  __shared__ __attribute__((aligned(16))) char stages[2 * kStageBytes];
+  __shared__ int s_pos[kRows];      // position of each query row, -1 for rows without a token
+  __shared__ float s_slope[kRows];  // its distance bias in score units
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15;
+  const int g = lane >> 4;
+  const int b = blockIdx.x / p.num_kv_heads;
+  const int kvh = blockIdx.x % p.num_kv_heads;
+  // the last row tiles see the most keys: first
+  const int r0 = (gridDim.y - 1 - blockIdx.y) * kRows;
+
+  const Row row = row_of(p, b);
+  int lo, hi;
+  row_positions(p, row, r0, r0 + kRows - 1, lo, hi);
+  const Span span = span_of(p, row, lo, hi);
+  int first = 0, n = span.n;
+  if (p.part_o) {  // this workgroup's part of the key tiles; the other kernel knows of empty ones
+    const int size = part_size(p, span.n);
+    first = min((int)blockIdx.z * size, span.n);
+    n = min(size, span.n - first);
+    if (n == 0) return;
+  }
+
+  // The table entry of key `lane` of key tile i, -1 where it is not to be read.
+  auto entry_of = [&](int i) -> int {
+    const int key = span.tile(first + i) * kKTile + lane;
+    const int blk = div_by(key, p.block_div);
+    return i < n && key < row.len && blk < p.max_blocks_per_seq
+               ? p.block_table[(int64_t)b * p.bt_stride + blk] : -1;
+  };
+  auto pool_row = [&](int i, int entry) -> int {
+    const int key = span.tile(first + i) * kKTile + lane;
+    const int slot = key - div_by(key, p.block_div) * p.block_size;
+    return entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
+  };
+  const char* kbase = (const char*)(p.k_cache + (int64_t)kvh * p.head_dim);
+  const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
+
+  int row_next = pool_row(0, entry_of(0));
+  issue_tile(p, kbase, vbase, stages, row_next, w, lane);
+  uint64_t keys = __builtin_amdgcn_ballot_w64(row_next >= 0), keys_next = 0;
+  row_next = pool_row(1, entry_of(1));
+  keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
+  issue_tile(p, kbase, vbase, stages + kStageBytes, row_next, w, lane);
+  int entry = entry_of(2);
+
+  // Q^T fragments: MFMA i takes d = 32 i + 8 g + s in reduction slot 8 g + s.
+  half8 qf[NB][4];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int r = r0 + kRowsPerWave * w + 16 * j + col;
+    const int t = div_by(r, p.group_div);
+    const int h = kvh * p.group + r - t * p.group;
+    const int pos = row.start + t;
+    const bool ok = t < p.chunk && pos >= 0 && pos < row.len;
+    const half_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)(ok ? t : 0) * p.q_st + (int64_t)h * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (ok && !p.q_zero && 32 * i + 8 * g < p.head_dim) v = *(const u32x4*)(src + 32 * i + 8 * g);
+      qf[j][i] = as_half8(v ^ p.q_sign);
+    }
+    if (g == 0) {
+      s_pos[kRowsPerWave * w + 16 * j + col] = ok ? pos : -1;
+      if (kMod & kBias) s_slope[kRowsPerWave * w + 16 * j + col] = p.slopes[h] * p.slope_mul;
+    }
+  }
+  const int* w_pos = s_pos + kRowsPerWave * w;
+  const float* w_slope = s_slope + kRowsPerWave * w;
+  int wlo, whi;  // positions of this wave's tokens
+  row_positions(p, row, r0 + kRowsPerWave * w, r0 + kRowsPerWave * (w + 1) - 1, wlo, whi);
+
+  float t_run[NB];
+  floatx4 acc[NB][9];  // O^T columns 16dt .. 16dt + 15 (dt < 8), sum of P (dt = 8)
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    t_run[j] = kNegBig;
+#pragma unroll
+    for (int dt = 0; dt < 9; ++dt) acc[j][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  stage_barrier();
+
+  // Tile i lies in stage i % 2.  While it is consumed, tile i + 1 is copied into the other stage
+  // (whose readers have passed the last barrier) and the table entries of tile i + 2 are read.
+  for (int i = 0; i < n; ++i) {
+    char* cur = stages + (i & 1) * kStageBytes;
+    if (i > 0) {
+      row_next = pool_row(i + 1, entry);
+      keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
+      entry = entry_of(i + 2);
+      issue_tile(p, kbase, vbase, stages + ((i + 1) & 1) * kStageBytes, row_next, w, lane);
+    }
+    const int k0 = span.tile(first + i) * kKTile;
+    const int k1 = k0 + kKTile - 1;
+    const bool any = wlo <= whi && (k0 < row.prefix || (k0 <= whi && k1 > wlo - p.window));
+    if (any) {
+      const bool all = keys == ~0ull && (k1 < row.prefix || (k1 <= wlo && k0 > whi - p.window));
+      consume<NB, kMod>(p, cur, k0, keys, !all, row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
+    }
+    keys = keys_next;
+    stage_barrier();
+  }
+
+  if (p.part_o) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      const int r = r0 + kRowsPerWave * w + 16 * j + col;
+      if (w_pos[16 * j + col] < 0) continue;
+      const int t = div_by(r, p.group_div);
+      const int64_t slot =
+          (((int64_t)b * p.chunk + t) * p.num_q_heads + kvh * p.group + r - t * p.group) *
+              p.max_splits + blockIdx.z;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt)
+        *(floatx4*)(p.part_o + slot * kHeadDim + 16 * dt + 4 * g) = acc[j][dt];
+      if (g == 0) {
+        p.part_ml[slot * 2] = __builtin_fmaf(t_run[j], p.scale_log2, -p.lazy_log2);
+        p.part_ml[slot * 2 + 1] = acc[j][8][0];
+      }
+    }
+    return;
+  }
+
+  // Normalise; the rows go through this wave's part of the stages (idle since the last barrier)
+  // so that each store instruction writes whole rows.  Rows are padded to 272 bytes: the 16
+  // rows of one write land in distinct banks.
+  constexpr int kORow = 272;
+  static_assert(kWaves * kRowsPerWave * kORow <= 2 * kStageBytes, "output rows fit the stages");
+  char* ostage = stages + w * kRowsPerWave * kORow;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const float l = acc[j][8][0];
+    const float inv = w_pos[16 * j + col] >= 0 && __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
+    char* orow = ostage + (16 * j + col) * kORow + 8 * g;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) *(half4*)(orow + 32 * dt) = to_half4(acc[j][dt] * inv);
+  }
+  wave_lds_sync();
+  const int r4 = lane >> 4, c16 = lane & 15;
+#pragma unroll
+  for (int rr = 0; rr < kRowsPerWave / 4; ++rr) {
+    const int rl = 4 * rr + r4;
+    const int r = r0 + kRowsPerWave * w + rl;
+    const int t = div_by(r, p.group_div);
+    const int h = kvh * p.group + r - t * p.group;
+    const u32x4 v = *(const u32x4*)(ostage + rl * kORow + 16 * c16);
+    if (t < p.chunk && c16 < p.d_chunks)
+      *(u32x4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * c16) = v;
+  }
+}
+
+// Adds the parts of each query row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  32 lanes a
+// row, four columns a lane.  Rows without a token, and rows that see no key, give zeros.
+constexpr int kMergeRows = 8;
+__global__ __launch_bounds__(32 * kMergeRows) void merge_kernel(Params p) {
+  const int64_t r = (int64_t)blockIdx.x * kMergeRows + (threadIdx.x >> 5);
+  const int d = 4 * (threadIdx.x & 31);
+  if (r >= (int64_t)p.batch * p.chunk * p.num_q_heads) return;
+  const int h = (int)(r % p.num_q_heads);
+  const int64_t bt = r / p.num_q_heads;
+  const int t = (int)(bt % p.chunk);
+  const int b = (int)(bt / p.chunk);
+  const Row row = row_of(p, b);
+  const int pos = row.start + t;
+  int parts = 0;
+  if (pos >= 0 && pos < row.len) {
+    const int r0 = (t * p.group + h % p.group) / p.rows_per_tile * p.rows_per_tile;
+    int lo, hi;
+    row_positions(p, row, r0, r0 + p.rows_per_tile - 1, lo, hi);
+    const int n = span_of(p, row, lo, hi).n;
+    const int size = part_size(p, n);
+    parts = (n + size - 1) / size;
+  }
+  float m = kNegBig, l = 0.f;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s = 0; s < parts; ++s) {
+    const int64_t slot = r * p.max_splits + s;
+    const float ls = p.part_ml[slot * 2 + 1];
+    if (__builtin_bit_cast(uint32_t, ls) == 0) continue;  // a part without a visible key
+    const float ms = p.part_ml[slot * 2];
+    const floatx4 os = *(const floatx4*)(p.part_o + slot * kHeadDim + d);
+    const float mn = fmaxf(m, ms);
+    const float a = fast_exp2(m - mn), e = fast_exp2(ms - mn);
+    l = l * a + ls * e;
+    o = o * a + os * e;
+    m = mn;
+  }
+  const float inv = __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
+  if (d < p.head_dim)
+    *(half4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + d) =
+        to_half4(o * inv);
+}
+
+// How a call is cut: row blocks per wave, row tiles per (row, kv head), parts per row tile.
+constexpr int64_t kSlots = 512;  // workgroups resident at once: two per CU
+constexpr int kMinPart = 4;
+struct Plan {
+  int nb;
+  int64_t row_tiles, splits;
+};
+static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads,
+                 int64_t num_tokens) {
+  const int64_t rows = chunk * (num_q_heads / num_kv_heads);
+  Plan pl;
+  pl.nb = (int)std::min<int64_t>((rows + 63) / 64, kMaxNb);
+  pl.row_tiles = (rows + 64 * pl.nb - 1) / (64 * pl.nb);
+  const int64_t wgs = batch * num_kv_heads * pl.row_tiles;
+  const int64_t tiles = (num_tokens + kKTile - 1) / kKTile;
+  pl.splits = std::max<int64_t>(std::min(kSlots / wgs, (tiles + kMinPart - 1) / kMinPart), 1);
+  return pl;
+}
+
+// Bytes of `splits` parts a query row.
+static size_t part_bytes(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t splits) {
+  return splits <= 1 ? 0 : (size_t)(batch * chunk * num_q_heads * splits * (kHeadDim + 2)) * sizeof(float);
+}
+
+static bool sizes_ok(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads) {
+  return batch >= 0 && chunk >= 0 && num_q_heads > 0 && num_kv_heads > 0 &&
+         num_q_heads % num_kv_heads == 0;
+}
+
+template <int kMod>
+static void launch(int nb, dim3 grid, hipStream_t st, const Params& p) {
+  const dim3 block(kThreads);
+  if (nb == 1)
+    hipLaunchKernelGGL((chunk_kernel<1, kMod>), grid, block, 0, st, p);
+  else if (nb == 2)
+    hipLaunchKernelGGL((chunk_kernel<2, kMod>), grid, block, 0, st, p);
+  else
+    hipLaunchKernelGGL((chunk_kernel<3, kMod>), grid, block, 0, st, p);
+}
+
+}  // namespace chunk
+}  // namespace fi
+
+extern "C" size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t num_new,
+                                                          int64_t num_q_heads, int64_t num_kv_heads,
+                                                          int64_t max_num_tokens, int64_t head_dim) {
+  using namespace fi::chunk;
+  if (!sizes_ok(batch, num_new, num_q_heads, num_kv_heads) || batch == 0 || num_new == 0 ||
+      max_num_tokens <= 0 || max_num_tokens > kMaxTokens || !fi::head_dim_ok(head_dim) ||
+      batch > 0x7fffffff || num_new > 0x7fffffff / num_q_heads)
+    return 0;
+  return part_bytes(batch, num_new, num_q_heads,
+                    plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens).splits);
+}
+
+extern "C" int fi_paged_chunk_attention_fwd(
+    const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh, const void* k_cache, const void* v_cache,
+    int64_t num_pool_blocks, int64_t block_size, int64_t num_kv_heads, const int32_t* block_table,
+    int64_t bt_stride, int64_t max_blocks_per_seq, const int32_t* start_positions,
+    const int32_t* context_lens, int64_t num_tokens, void* o, int64_t o_sb, int64_t o_st, int64_t o_sh,
+    int64_t batch, int64_t num_new, int64_t num_q_heads, int64_t head_dim, float sm_scale, float softcap,
+    const float* alibi_slopes, int64_t window, const int32_t* prefix_lens, void* workspace,
+    size_t workspace_bytes, void* stream) {
+  using namespace fi;
+  using namespace fi::chunk;
+  static const char* fn = "fi_paged_chunk_attention_fwd";
+  clear_error();
+  if (!head_dim_ok(head_dim)) {
+    set_error("%s: head_dim %lld not supported (a multiple of 8 up to %d)", fn, (long long)head_dim,
+              kHeadDim);
+    return FI_ERR_UNSUPPORTED;
+  }
+  if (!sizes_ok(batch, num_new, num_q_heads, num_kv_heads) || num_tokens < 0 || num_pool_blocks < 0 ||
+      max_blocks_per_seq < 0) {
+    set_error("%s: invalid sizes (batch %lld, new tokens %lld, heads %lld/%lld, tokens %lld)", fn,
+              (long long)batch, (long long)num_new, (long long)num_q_heads, (long long)num_kv_heads,
+              (long long)num_tokens);
+    return FI_ERR_INVALID;
+  }
+  if (block_size <= 0) {
+    set_error("%s: block_size %lld must be positive", fn, (long long)block_size);
+    return FI_ERR_INVALID;
+  }
+  if (window < 0) {
+    set_error("%s: window %lld must be positive, or 0 for none", fn, (long long)window);
+    return FI_ERR_INVALID;
+  }
+  const float cap_arg = softcap != 0.f ? sm_scale / softcap : 0.f;
+  if (!std::isfinite(sm_scale) || !std::isfinite(softcap) || softcap < 0.f || !std::isfinite(cap_arg)) {
+    set_error("%s: sm_scale %g and softcap %g must be finite, the cap positive (0 for none)", fn,
+              (double)sm_scale, (double)softcap);
+    return FI_ERR_INVALID;
+  }
+  if (batch == 0 || num_new == 0) return FI_OK;
+  if (num_tokens > kMaxTokens || num_pool_blocks > 0x7fffffff / block_size ||
+      max_blocks_per_seq > 0x7fffffff || batch > 0x7fffffff / num_kv_heads ||
+      num_new > 0x7fffffff / num_q_heads / 2 ||
+      batch * num_new > (int64_t)0x7fffffff * kMergeRows / num_q_heads) {
+    set_error("%s: sizes too large (at most %lld tokens a row, 2^31 pool slots)", fn,
+              (long long)kMaxTokens);
+    return FI_ERR_UNSUPPORTED;
+  }
+  // an empty bound reads no table and no pool
+  if (!q || !o || (num_tokens > 0 && (!k_cache || !v_cache || !block_table))) {
+    set_error("%s: null pointer", fn);
+    return FI_ERR_INVALID;
+  }
+  if ((((uintptr_t)q | (uintptr_t)o | (uintptr_t)k_cache | (uintptr_t)v_cache) & 15u) ||
+      (q_sb | q_st | q_sh | o_sb | o_st | o_sh) % 8 != 0) {
+    set_error("%s: rows must be 16-byte aligned (strides multiple of 8)", fn);
+    return FI_ERR_INVALID;
+  }
+
+  Params p = {};
+  p.q = (const half_t*)q;
+  p.q_sb = q_sb; p.q_st = q_st; p.q_sh = q_sh;
+  p.k_cache = (const half_t*)k_cache;
+  p.v_cache = (const half_t*)v_cache;
+  p.num_pool_blocks = (int)num_pool_blocks;
+  p.block_size = (int)block_size;
+  p.block_div = fast_div((uint32_t)block_size);
+  p.num_kv_heads = (int)num_kv_heads;
+  p.row_bytes = num_kv_heads * head_dim * 2;
+  p.block_table = block_table;
+  p.bt_stride = bt_stride;
+  p.max_blocks_per_seq = (int)max_blocks_per_seq;
+  p.start_positions = start_positions;
+  p.context_lens = context_lens;
+  p.num_tokens = (int)(max_blocks_per_seq < num_tokens / block_size + 1
+                           ? std::min(num_tokens, max_blocks_per_seq * block_size) : num_tokens);
+  p.o = (half_t*)o;
+  p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
+  p.batch = (int)batch;
+  p.chunk = (int)num_new;
+  p.num_q_heads = (int)num_q_heads;
+  p.group = (int)(num_q_heads / num_kv_heads);
+  p.group_div = fast_div((uint32_t)p.group);
+  p.head_dim = (int)head_dim;
+  p.d_chunks = (int)(head_dim / 8);
+  if (softcap > 0.f) {
+    p.scale_log2 = 1.f;
+    p.cap_arg = cap_arg;
+    p.cap_log2 = softcap * kLog2e;
+  } else {
+    // scores are masked before they are scaled and -inf * 0 is NaN: a zero scale runs as unit
+    // scale on a Q of zeros; a negative one on a negated Q
+    p.q_zero = sm_scale == 0.f;
+    p.q_sign = sm_scale < 0.f ? 0x80008000u : 0u;
+    p.scale_log2 = p.q_zero ? kLog2e : std::fabs(sm_scale) * kLog2e;
+  }
+  p.lazy_raw = kLazyLog2 / p.scale_log2;
+  p.lazy_log2 = p.lazy_raw * p.scale_log2;
+  p.slopes = alibi_slopes;
+  p.slope_mul = kLog2e / p.scale_log2;
+  p.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
+  p.prefix_lens = prefix_lens;
+
+  const Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens);
+  const int64_t one = (int64_t)part_bytes(batch, num_new, num_q_heads, 2) / 2;
+  const int64_t room = workspace ? (int64_t)std::min<size_t>(workspace_bytes, (size_t)1 << 62) / one : 0;
+  const int64_t splits = std::min(pl.splits, std::max<int64_t>(room, 1));
+  p.rows_per_tile = 64 * pl.nb;
+  p.max_splits = (int)splits;
+  p.min_part = kMinPart;
+  const int64_t rows = batch * num_new * num_q_heads;
+  if (splits > 1) {
+    if ((uintptr_t)workspace & 15u) {
+      set_error("%s: workspace must be 16-byte aligned", fn);
+      return FI_ERR_INVALID;
+    }
+    p.part_o = (float*)workspace;
+    p.part_ml = p.part_o + rows * splits * kHeadDim;
+  }
+  if (pl.row_tiles > 65535) {
+    set_error("%s: too many new tokens (%lld)", fn, (long long)num_new);
+    return FI_ERR_UNSUPPORTED;
+  }
+  const dim3 grid((unsigned)(batch * num_kv_heads), (unsigned)pl.row_tiles, (unsigned)splits);
+  const hipStream_t st = (hipStream_t)stream;
+  switch ((softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0)) {
+    case 0: launch<0>(pl.nb, grid, st, p); break;
+    case kCap: launch<kCap>(pl.nb, grid, st, p); break;
+    case kBias: launch<kBias>(pl.nb, grid, st, p); break;
+    default: launch<kCap | kBias>(pl.nb, grid, st, p); break;
+  }
+  const int rc = check_launch(fn);
+  if (rc != FI_OK || splits == 1) return rc;
+  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((rows + kMergeRows - 1) / kMergeRows)),
+                     dim3(32 * kMergeRows), 0, st, p);
+  return check_launch(fn);
+}

@@ -6,7 +6,8 @@ dequantization then runs inside the MFMA loop — or an fp16 ``[N, K]`` weight.
 ``quantize_int4_groupwise`` (loader.py:9-41) and ``dequantize_int4`` (the reference's
 ``_dequant_storage``, matmul.py:309-326) produce and expand the same wire format, bit for
 bit.  ``rms_norm`` is kernels/rms_norm.py's; ``rms_norm_int4_matmul`` is the norm of
-model.py:82 and the projection after it in one call.
+model.py:82 and the projection after it in one call; ``add_rms_norm`` the residual addition
+before a norm and the norm.
 """
 
 from __future__ import annotations
@@ -209,6 +210,44 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5) -> torch.
                                     out.data_ptr(), hidden, _lib.tensor_stream(x))
         _lib.check(rc, "rms_norm")
     return out.reshape(x.shape)
+
+
+def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
+                 eps: float = 1e-5, *, inplace: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """The residual addition and the norm of its result in one pass: ``h = x + residual`` (fp16,
+    rounded once) and ``rms_norm(h, weight, eps)``, for ``x`` and ``residual`` fp16 ``[...,
+    hidden]`` of one shape.  Returns ``(normed, h)``.  With ``inplace`` h is written into
+    ``residual`` (which then needs rows the kernel can write: unit inner stride, 16-byte aligned,
+    one row stride) and returned as that tensor."""
+    _need_cuda("x", x)
+    _need_cuda("residual", residual)
+    hidden = x.shape[-1]
+    if residual.shape != x.shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
+    if residual.get_device() != x.get_device():
+        raise RuntimeError("residual must be on the same device as x")
+    if x.dtype is not torch.float16 or residual.dtype is not torch.float16:
+        raise TypeError(f"x and residual must be float16, got {x.dtype} / {residual.dtype}")
+    if weight.shape != (hidden,):
+        raise ValueError(f"weight {tuple(weight.shape)} does not match hidden {hidden}")
+    wt = _norm_weight(weight, x)
+    x2, x_stride, x_ptr = _rows16(x.reshape(-1, hidden), 2)
+    r2, r_stride, r_ptr = _rows16(residual.reshape(-1, hidden), 2)
+    rows = x2.shape[0]
+    out = torch.empty(rows, hidden, dtype=torch.float16, device=x.device)
+    if inplace:
+        if rows and r_ptr != residual.data_ptr():
+            raise ValueError("an in-place residual needs 16-byte aligned rows at one row stride")
+        h, h_stride, h_ptr = residual, r_stride, r_ptr
+    else:
+        h = torch.empty(x.shape, dtype=torch.float16, device=x.device)
+        h_stride, h_ptr = hidden, h.data_ptr()
+    if rows:
+        rc = _lib.calls().fi_add_rmsnorm(x_ptr, x_stride, r_ptr, r_stride, rows, hidden,
+                                        wt.data_ptr(), float(eps), h_ptr, h_stride, out.data_ptr(),
+                                        hidden, _lib.tensor_stream(x))
+        _lib.check(rc, "add_rms_norm")
+    return out.reshape(x.shape), h
 
 
 def rms_norm_int4_matmul(x: torch.Tensor, norm_weight: torch.Tensor, w, eps: float = 1e-5,

@@ -12,6 +12,9 @@
  *   fi_paged_attention_fwd   single-query attention over the paged KV pool
  *                            replaces kernels/attention.py:191-233 (paged_attention,
  *                            launching _paged_attention_kernel :116-188).
+ *   fi_paged_chunk_attention_fwd
+ *                            attention of several new tokens per sequence over the pool, with
+ *                            optional capped scores, distance bias, window and prefix.
  *   fi_kv_store              scatter of K/V rows into the paged pool
  *                            replaces model.py:162-183 (_store_kv_prefill copies),
  *                            model.py:185-201 (_store_kv_decode copies) and
@@ -176,6 +179,51 @@ FI_API int fi_paged_attention_fwd_noalloc(const void* q, int64_t q_sb, int64_t q
                                    void* stream);
 
 /*
+ * Attention of a chunk of new tokens over the paged pool: what continues sequences by several
+ * tokens (a prompt prefilled in pieces or behind a cached beginning, drafted tokens), and single
+ * tokens with the score options below.  No counterpart in the reference, which prefills whole
+ * prompts (kernels/attention.py:80-113) and decodes single tokens (:191-233).  The chunk's own K
+ * and V have to be in the pool already (fi_rope_store_kv or fi_kv_store before this call).
+ *
+ *   q, o        : [batch, num_new, num_q_heads, head_dim], strides (q_sb, q_st, q_sh) /
+ *                 (o_sb, o_st, o_sh); rows 16-byte aligned (strides multiples of 8)
+ *   k/v_cache, block_table, context_lens, num_tokens: as fi_paged_attention_fwd; a row's length
+ *                 counts its new tokens and is also bounded by its table's max_blocks_per_seq
+ *                 blocks; at most 2^22 tokens a row
+ *   start_positions: int32[batch], the position of each row's first new token (fi_kv_append's
+ *                 start_pos_out); NULL -> the chunk is the last num_new tokens of the row.
+ *   Token t of row b stands at pos = start + t and sees key j (j < length, table entry inside the
+ *   pool) when j < prefix or pos - window < j <= pos.  Tokens whose pos is negative or not below
+ *   the row's length (the padding of a batch with fewer new tokens in some rows), and tokens that
+ *   see no key, give zeros.  What the pool holds where a token does not look, infinities and
+ *   NaN included, does not reach it.
+ *   softcap     : 0, or cap > 0: x = cap * tanh(x / cap) for the scaled scores x = sm_scale * q.k
+ *   alibi_slopes: NULL, or fp32[num_q_heads]: x -= slope * |pos - j|, after the cap
+ *   window      : 0 for no window, else the number of positions a token sees up to its own
+ *   prefix_lens : NULL, or int32[batch]: positions that every token of the row sees, before and
+ *                 behind it (a prefix mask; with a window, tokens that stay visible)
+ *   workspace   : fi_paged_chunk_attention_workspace_size(batch, num_new, num_q_heads,
+ *                 num_kv_heads, num_tokens, head_dim) bytes, 16-byte aligned; it needs no
+ *                 initialisation.  With less (or NULL) the call runs with fewer parts, slower.
+ *                 Calls that overlap in time must not share it.
+ */
+FI_API size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t num_new,
+                                               int64_t num_q_heads, int64_t num_kv_heads,
+                                               int64_t max_num_tokens, int64_t head_dim);
+FI_API int fi_paged_chunk_attention_fwd(const void* q, int64_t q_sb, int64_t q_st, int64_t q_sh,
+                                 const void* k_cache, const void* v_cache,
+                                 int64_t num_pool_blocks, int64_t block_size,
+                                 int64_t num_kv_heads, const int32_t* block_table,
+                                 int64_t bt_stride, int64_t max_blocks_per_seq,
+                                 const int32_t* start_positions, const int32_t* context_lens,
+                                 int64_t num_tokens, void* o, int64_t o_sb, int64_t o_st,
+                                 int64_t o_sh, int64_t batch, int64_t num_new,
+                                 int64_t num_q_heads, int64_t head_dim, float sm_scale,
+                                 float softcap, const float* alibi_slopes, int64_t window,
+                                 const int32_t* prefix_lens, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
+/*
  * Scatter K/V rows into the paged pool (byte-exact copies).
  * Replaces the slice copies of model.py:176-183 (prefill), model.py:196-201 (decode)
  * and kv_cache.py:69-103.
@@ -329,6 +377,19 @@ FI_API int fi_int4_matmul(const void* x, int64_t x_stride, int64_t M, int64_t K,
  */
 FI_API int fi_rmsnorm(const void* x, int64_t x_stride, int64_t M, int64_t hidden,
                const void* weight, float eps, void* out, int64_t out_stride, void* stream);
+
+/*
+ * A block's output added to the residual stream, and the RMSNorm of the sum (the one before the
+ * next projection, as at model.py:82), in one pass:
+ * h_out[m] = fp16(x[m] + residual[m]); out[m] = fi_rmsnorm(h_out[m]).
+ *   x, residual, h_out, out: fp16 [M, hidden] (row strides in elements, 16-byte aligned rows);
+ *   weight: fp16 [hidden]; hidden a multiple of 8 up to 2^24, fewer than 2^24 rows.
+ *   h_out may be residual or x, and out may be the other of them (same rows and stride); h_out
+ *   and out must not overlap.
+ */
+FI_API int fi_add_rmsnorm(const void* x, int64_t x_stride, const void* residual,
+                   int64_t res_stride, int64_t M, int64_t hidden, const void* weight, float eps,
+                   void* h_out, int64_t h_stride, void* out, int64_t out_stride, void* stream);
 
 /*
  * rms_norm followed by int4_matmul as one call (model.py:82 then :87 / :91-93): out =
