@@ -125,17 +125,35 @@ __device__ __forceinline__ void row_positions(const Params& p, const Row& row, i
   hi = min(row.start + min(div_by(r1, p.group_div), p.chunk - 1), row.len - 1);
 }
 
-// The key tiles a row tile visits: tiles 0 .. n_pre - 1 (prefix), then from `from` on.
+// The key tiles a row tile visits: tiles 0 .. n_pre - 1 (prefix), then the causal ones from `from`
+// on.  They are taken in an order that puts those first in which some row may not see some key
+// (the ends of the window and of the prefix, the diagonal), so that the others run in a loop
+// without masks: list places [tail, n), [full_pre, head), then [0, full_pre), [head, tail).
 struct Span {
   int n_pre, from, n;
-  __device__ __forceinline__ int tile(int i) const { return i < n_pre ? i : from + i - n_pre; }
+  int full_pre, head, tail;
+  __device__ __forceinline__ int masked() const { return n - tail + head - full_pre; }
+  __device__ __forceinline__ int tile(int i) const {  // of place i in the order
+    int at = i + tail;
+    if (i >= n - tail) at = full_pre + i - (n - tail);
+    if (i >= masked()) at = i - masked();
+    if (i >= masked() + full_pre) at = head + i - masked() - full_pre;
+    return at < n_pre ? at : from + at - n_pre;
+  }
 };
 __device__ __forceinline__ Span span_of(const Params& p, const Row& row, int lo, int hi) {
   Span s;
   s.n_pre = (row.prefix + kKTile - 1) / kKTile;
   s.from = max(max(lo - p.window + 1, 0) / kKTile, s.n_pre);
-  s.n = s.n_pre + max((hi + kKTile) / kKTile - s.from, 0);
-  if (lo > hi) s.n = 0;
+  const int end = max((hi + kKTile) / kKTile, s.from);
+  s.n = s.n_pre + end - s.from;
+  s.full_pre = row.prefix / kKTile;
+  // causal tiles that every row sees whole: behind hi - window, and up to lo
+  const int a = min(max(hi >= p.window ? (hi - p.window) / kKTile + 1 : 0, s.from), end);
+  const int e = max(min((lo + 1) / kKTile, end), a);
+  s.head = s.n_pre + a - s.from;
+  s.tail = s.n_pre + e - s.from;
+  if (lo > hi) s.n = s.full_pre = s.head = s.tail = 0;
   return s;
 }
 __device__ __forceinline__ int part_size(const Params& p, int n) {
@@ -312,12 +330,12 @@ __device__ __forceinline__ float capped(const Params& p, float s, bool series) {
   return x;
 }
 
-// One resident tile (keys k0 .. k0 + 63) for this wave's rows.  s_pos: positions of the
-// workgroup's rows; keys: bit k is set when key k0 + k is before the row's length and in the
-// pool; masked: some row does not see some key.
-template <int NB, int kMod>
+// One resident tile (keys k0 .. k0 + 63) for this wave's rows.  s_pos, s_slope: of the wave's rows;
+// keys: bit k is set when key k0 + k is before the row's length and in the pool; kMasked: some
+// row may not see some key.
+template <int NB, int kMod, bool kMasked>
 __device__ __forceinline__ void consume(const Params& p, const char* stage, int k0, uint64_t keys,
-                                        bool masked, int prefix, const int* s_pos,
+                                        int prefix, const int* s_pos,
                                         const float* s_slope, int col, int g,
                                         const half8 (&qf)[NB][4], float (&t_run)[NB],
                                         floatx4 (&acc)[NB][9]) {
@@ -352,7 +370,7 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
             if (kMod & kBias) s[j][t][r] += bias(j, t, r);
           }
     }
-    if (masked) {
+    if (kMasked) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         const int pos = s_pos[16 * j + col];
@@ -366,6 +384,15 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
             if (!see) s[j][t][r] = -__builtin_inff();
           }
       }
+    } else if (keys != ~0ull) {  // missing table entries
+      const uint32_t bits = (uint32_t)(keys >> (32 * c)) >> (4 * g);
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (!((bits >> (16 * t + r)) & 1)) s[j][t][r] = -__builtin_inff();
     }
     // Online softmax with a lazily moved reference max, kept as the threshold t = max + slack in
     // score units: it moves only when a score exceeds it (p <= 2^8, exact in fp16; sums in fp32).
@@ -400,7 +427,7 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
         for (int r = 0; r < 4; ++r)
           pf[j][4 * t + r] = (half_t)fast_exp2(__builtin_fmaf(s[j][t][r], p.scale_log2, -mc));
     }
-    if (masked && !v_finite(vs, c, col, g))
+    if (kMasked && !v_finite(vs, c, col, g))
       pv_slice_careful<NB>(vs, c, col, g, pf, acc);
     else
       pv_slice<NB>(vs, c, col, g, pf, acc);
@@ -498,21 +525,28 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
 
   // Tile i lies in stage i % 2.  While it is consumed, tile i + 1 is copied into the other stage
   // (whose readers have passed the last barrier) and the table entries of tile i + 2 are read.
-  for (int i = 0; i < n; ++i) {
-    char* cur = stages + (i & 1) * kStageBytes;
-    if (i > 0) {
-      row_next = pool_row(i + 1, entry);
-      keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
-      entry = entry_of(i + 2);
-      issue_tile(p, kbase, vbase, stages + ((i + 1) & 1) * kStageBytes, row_next, w, lane);
-    }
+  auto copy_next = [&](int i) {
+    if (i == 0) return;  // the first two are on their way
+    row_next = pool_row(i + 1, entry);
+    keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
+    entry = entry_of(i + 2);
+    issue_tile(p, kbase, vbase, stages + ((i + 1) & 1) * kStageBytes, row_next, w, lane);
+  };
+  int i = 0;
+  for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
+    copy_next(i);
     const int k0 = span.tile(first + i) * kKTile;
-    const int k1 = k0 + kKTile - 1;
-    const bool any = wlo <= whi && (k0 < row.prefix || (k0 <= whi && k1 > wlo - p.window));
-    if (any) {
-      const bool all = keys == ~0ull && (k1 < row.prefix || (k1 <= wlo && k0 > whi - p.window));
-      consume<NB, kMod>(p, cur, k0, keys, !all, row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
-    }
+    if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
+      consume<NB, kMod, true>(p, stages + (i & 1) * kStageBytes, k0, keys, row.prefix, w_pos, w_slope, col,
+                              g, qf, t_run, acc);
+    keys = keys_next;
+    stage_barrier();
+  }
+  for (; i < n; ++i) {
+    copy_next(i);
+    if (wlo <= whi)
+      consume<NB, kMod, false>(p, stages + (i & 1) * kStageBytes, span.tile(first + i) * kKTile, keys,
+                               row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
     keys = keys_next;
     stage_barrier();
   }
