@@ -39,6 +39,8 @@ constexpr int kMaxNb = 3;
 constexpr float kLazyLog2 = 8.f;  // the reference max may lag the true max by 2^8
 constexpr int kNoWindow = 0x3fffffff;
 constexpr int64_t kMaxTokens = (int64_t)1 << 22;
+constexpr int kMinPart = 2;      // key tiles of the smallest part
+constexpr int64_t kSlots = 512;  // workgroups resident at once (two per CU): parts aimed at
 // Largest cap whose tanh is taken from exp2 alone: its absolute error, about 2e-7, times the
 // cap is an error of the logit, here 1e-4.
 constexpr float kExpCap = 500.f;
@@ -89,16 +91,18 @@ struct Params {
   float lazy_log2;    // lazy_raw * scale_log2
   uint32_t q_sign;    // 0x80008000: Q negated (negative sm_scale without a cap)
   int q_zero;         // sm_scale == 0 without a cap: Q read as zeros
-  float cap_arg;      // sm_scale / cap
+  float cap_exp;      // sm_scale / cap * 2 log2(e)
   float cap_log2;     // cap * log2(e)
   const float* slopes;
   float slope_mul;    // slope unit -> score unit
   int window;
   const int32_t* prefix_lens;
-  int rows_per_tile;  // 64 * NB
-  int max_splits;
-  int min_part;       // key tiles of the smallest part
-  float* part_o;      // [batch * chunk * num_q_heads][max_splits][128]; null: write o
+  int tile_rows;      // query rows of a row tile, 64 * NB
+  FastDiv tile_div;
+  int row_tiles;      // of each (batch row, kv head): ceil(chunk * group / tile_rows)
+  int target;         // parts aimed at, all kv heads together
+  int part_rows;      // min(tile_rows, chunk * group): rows of a part's results
+  float* part_o;      // [parts, num_kv_heads][part_rows][128]; null: no parts, write o
   float* part_ml;     // [...][2]: reference max (log2 units), sum
 };
 
@@ -156,8 +160,74 @@ __device__ __forceinline__ Span span_of(const Params& p, const Row& row, int lo,
   if (lo > hi) s.n = s.full_pre = s.head = s.tail = 0;
   return s;
 }
-__device__ __forceinline__ int part_size(const Params& p, int n) {
-  return max((n + p.max_splits - 1) / p.max_splits, p.min_part);
+// The row tiles of a batch row that hold tokens (first .. first + count - 1), and the key tiles
+// of the last of them.
+struct RowTiles {
+  int first, count, n;
+};
+__device__ __forceinline__ RowTiles row_tiles_of(const Params& p, const Row& row) {
+  const int t0 = max(-row.start, 0), t1 = min(row.len - row.start, p.chunk);
+  RowTiles r = {0, 0, 0};
+  if (t0 < t1) {
+    r.first = div_by(t0 * p.group, p.tile_div);
+    const int last = div_by(t1 * p.group - 1, p.tile_div);
+    r.count = last - r.first + 1;
+    int lo, hi;
+    row_positions(p, row, last * p.tile_rows, (last + 1) * p.tile_rows - 1, lo, hi);
+    r.n = span_of(p, row, lo, hi).n;
+  }
+  return r;
+}
+
+// Every workgroup finds its part by itself, from the lengths on the device: the part size is all
+// key tiles to visit over the parts aimed at (kMinPart at least), each row tile of batch row b is
+// cut into parts(b) = ceil(its longest list / size) equal pieces, and the work list is, for each
+// b, its parts (row tile fastest, so that neighbours read the same keys), then its row tiles
+// without tokens, one each.  `size` and `before` (list entries of earlier batch rows) for row b;
+// with `item` >= 0, b is looked up from the list place.  Wave-wide; lanes hold batch rows.
+struct Share {
+  int b, before, parts;
+};
+__device__ __forceinline__ int wave_sum(int v) {
+#pragma unroll
+  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+  return v;
+}
+__device__ __forceinline__ Share find_share(const Params& p, int item, int b, int lane) {
+  auto tiles_of = [&](int i) { return i < p.batch ? row_tiles_of(p, row_of(p, i)) : RowTiles{0, 0, 0}; };
+  const RowTiles t0 = tiles_of(lane);
+  int total = t0.count * t0.n;
+  for (int i = lane + 64; i < p.batch; i += 64) {
+    const RowTiles t = tiles_of(i);
+    total += t.count * t.n;
+  }
+  total = wave_sum(total) * p.num_kv_heads;
+  const int size = max((total + p.target - 1) / p.target, kMinPart);
+  Share s = {-1, 0, 1};
+  int before = 0;
+  for (int i0 = 0; i0 < p.batch; i0 += 64) {
+    const RowTiles t = i0 == 0 ? t0 : tiles_of(i0 + lane);
+    const int parts = max((t.n + size - 1) / size, 1);
+    const int items = i0 + lane < p.batch ? t.count * parts + p.row_tiles - t.count : 0;
+    int upto = items;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int x = __shfl_up(upto, d);
+      if (lane >= d) upto += x;
+    }
+    upto += before;
+    const uint64_t hit =
+        item >= 0 ? __builtin_amdgcn_ballot_w64(upto > item) : (b >> 6) == (i0 >> 6) ? 1ull << (b & 63) : 0;
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      s.b = i0 + l;
+      s.before = __builtin_amdgcn_readlane(upto - items, l);
+      s.parts = __builtin_amdgcn_readlane(parts, l);
+      return s;
+    }
+    before = __builtin_amdgcn_readlane(upto, 63);
+  }
+  return s;
 }
 
 // LDS tile layouts, as in the prefill kernel: a K tile is 4 panels of 64 bytes per key (chunks
@@ -313,21 +383,20 @@ __device__ __forceinline__ void pv_slice_careful(const char* vs, int c, int col,
   for (int j = 0; j < NB; ++j) acc[j][8] = mfma16x16x32(ones, pf[j], acc[j][8]);
 }
 
-// x = cap_log2 * tanh(s * cap_arg), in log2 units.  tanh(y) = 1 - 2 / (1 + e^2y); for large caps,
-// where its absolute error would show, its series below 1/4 (the next term is under 2e-8).
-__device__ __forceinline__ float capped(const Params& p, float s, bool series) {
-  const float y = s * p.cap_arg;
-  const float e = fast_exp2(y * (2.f * kLog2e));
-  float x = __builtin_fmaf(-2.f * p.cap_log2, __builtin_amdgcn_rcpf(1.f + e), p.cap_log2);
-  if (series) {
-    const float z = y * y;
-    float t = __builtin_fmaf(z, 62.f / 2835.f, -17.f / 315.f);
-    t = __builtin_fmaf(z, t, 2.f / 15.f);
-    t = __builtin_fmaf(z, t, -1.f / 3.f);
-    t = __builtin_fmaf(z * y, t, y);
-    if (__builtin_fabsf(y) < 0.25f) x = p.cap_log2 * t;
-  }
-  return x;
+// x = cap_log2 * tanh(y), y = s * sm_scale / cap, in log2 units: tanh(y) = 1 - 2 / (1 + e^2y).
+__device__ __forceinline__ float capped(const Params& p, float s) {
+  const float e = fast_exp2(s * p.cap_exp);
+  return __builtin_fmaf(-2.f * p.cap_log2, __builtin_amdgcn_rcpf(1.f + e), p.cap_log2);
+}
+// The same for large caps, where the absolute error of that form would show: below 1/4 the series
+// (the next term is under 2e-8).
+__device__ __forceinline__ float capped_series(const Params& p, float s) {
+  const float y = s * (p.cap_exp * (0.5f / kLog2e)), z = y * y;
+  float t = __builtin_fmaf(z, 62.f / 2835.f, -17.f / 315.f);
+  t = __builtin_fmaf(z, t, 2.f / 15.f);
+  t = __builtin_fmaf(z, t, -1.f / 3.f);
+  t = __builtin_fmaf(z * y, t, y);
+  return __builtin_fabsf(y) < 0.25f ? p.cap_log2 * t : capped(p, s);
 }
 
 // One resident tile (keys k0 .. k0 + 63) for this wave's rows.  s_pos, s_slope: of the wave's rows;
@@ -361,14 +430,19 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
     if (kMod & kCap) {
       const bool series = p.cap_log2 > kExpCap * kLog2e;
 #pragma unroll
-      for (int j = 0; j < NB; ++j)
+      for (int j = 0; j < NB; ++j) {
+        if (series) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+          for (int e = 0; e < 8; ++e) s[j][e >> 2][e & 3] = capped_series(p, s[j][e >> 2][e & 3]);
+        } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            s[j][t][r] = capped(p, s[j][t][r], series);
-            if (kMod & kBias) s[j][t][r] += bias(j, t, r);
-          }
+          for (int e = 0; e < 8; ++e) s[j][e >> 2][e & 3] = capped(p, s[j][e >> 2][e & 3]);
+        }
+        if (kMod & kBias) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[j][e >> 2][e & 3] += bias(j, e >> 2, e & 3);
+        }
+      }
     }
     if (kMasked) {
 #pragma unroll
@@ -447,22 +521,37 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15;
   const int g = lane >> 4;
-  const int b = blockIdx.x / p.num_kv_heads;
   const int kvh = blockIdx.x % p.num_kv_heads;
-  // the last row tiles see the most keys: first
-  const int r0 = (gridDim.y - 1 - blockIdx.y) * kRows;
+  const int item = blockIdx.x / p.num_kv_heads;
+  int b, tile, part = 0, parts = 1;
+  if (p.part_o) {
+    const Share s = find_share(p, item, 0, lane);
+    if (s.b < 0) return;  // past the list
+    b = s.b;
+    const RowTiles rt = row_tiles_of(p, row_of(p, b));
+    int at = item - s.before;
+    if (at < rt.count * s.parts) {
+      part = at / rt.count;
+      parts = s.parts;
+      tile = rt.first + rt.count - 1 - (at - part * rt.count);
+    } else {  // a row tile without tokens
+      at -= rt.count * s.parts;
+      tile = at < rt.first ? at : at + rt.count;
+    }
+  } else {  // the last row tiles see the most keys: first
+    b = item % p.batch;
+    tile = p.row_tiles - 1 - item / p.batch;
+  }
+  const int r0 = tile * kRows;
 
   const Row row = row_of(p, b);
   int lo, hi;
   row_positions(p, row, r0, r0 + kRows - 1, lo, hi);
   const Span span = span_of(p, row, lo, hi);
-  int first = 0, n = span.n;
-  if (p.part_o) {  // this workgroup's part of the key tiles; the other kernel knows of empty ones
-    const int size = part_size(p, span.n);
-    first = min((int)blockIdx.z * size, span.n);
-    n = min(size, span.n - first);
-    if (n == 0) return;
-  }
+  const int size = (span.n + parts - 1) / parts;
+  const int first = min(part * size, span.n);
+  const int n = min(size, span.n - first);
+  if (parts > 1 && n == 0) return;  // a short list in few pieces: the other kernel reads no more
 
   // The table entry of key `lane` of key tile i, -1 where it is not to be read.
   auto entry_of = [&](int i) -> int {
@@ -551,15 +640,12 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     stage_barrier();
   }
 
-  if (p.part_o) {
+  if (parts > 1) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const int r = r0 + kRowsPerWave * w + 16 * j + col;
+      const int rl = kRowsPerWave * w + 16 * j + col;
       if (w_pos[16 * j + col] < 0) continue;
-      const int t = div_by(r, p.group_div);
-      const int64_t slot =
-          (((int64_t)b * p.chunk + t) * p.num_q_heads + kvh * p.group + r - t * p.group) *
-              p.max_splits + blockIdx.z;
+      const int64_t slot = (int64_t)blockIdx.x * p.part_rows + rl;
 #pragma unroll
       for (int dt = 0; dt < 8; ++dt)
         *(floatx4*)(p.part_o + slot * kHeadDim + 16 * dt + 4 * g) = acc[j][dt];
@@ -600,40 +686,47 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
 }
 
 // Adds the parts of each query row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  32 lanes a
-// row, four columns a lane.  Rows without a token, and rows that see no key, give zeros.
+// row, four columns a lane; grid (rows of a batch row, batch).  Batch rows that were not cut, and
+// rows without a token, were written by the kernel above.
 constexpr int kMergeRows = 8;
 __global__ __launch_bounds__(32 * kMergeRows) void merge_kernel(Params p) {
-  const int64_t r = (int64_t)blockIdx.x * kMergeRows + (threadIdx.x >> 5);
+  const int b = blockIdx.y;
+  const Share s = find_share(p, -1, b, threadIdx.x & 63);
+  if (s.parts <= 1) return;
+  const int r = blockIdx.x * kMergeRows + (threadIdx.x >> 5);  // (token, query head)
   const int d = 4 * (threadIdx.x & 31);
-  if (r >= (int64_t)p.batch * p.chunk * p.num_q_heads) return;
-  const int h = (int)(r % p.num_q_heads);
-  const int64_t bt = r / p.num_q_heads;
-  const int t = (int)(bt % p.chunk);
-  const int b = (int)(bt / p.chunk);
+  if (r >= p.chunk * p.num_q_heads) return;
+  const int t = r / p.num_q_heads;
+  const int h = r - t * p.num_q_heads;
   const Row row = row_of(p, b);
   const int pos = row.start + t;
-  int parts = 0;
-  if (pos >= 0 && pos < row.len) {
-    const int r0 = (t * p.group + h % p.group) / p.rows_per_tile * p.rows_per_tile;
-    int lo, hi;
-    row_positions(p, row, r0, r0 + p.rows_per_tile - 1, lo, hi);
-    const int n = span_of(p, row, lo, hi).n;
-    const int size = part_size(p, n);
-    parts = (n + size - 1) / size;
-  }
-  float m = kNegBig, l = 0.f;
+  const RowTiles rt = row_tiles_of(p, row);
+  const int kvh = div_by(h, p.group_div);
+  const int kr = t * p.group + h - kvh * p.group;
+  const int tile = div_by(kr, p.tile_div);
+  if (tile < rt.first || tile >= rt.first + rt.count) return;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < parts; ++s) {
-    const int64_t slot = r * p.max_splits + s;
-    const float ls = p.part_ml[slot * 2 + 1];
-    if (__builtin_bit_cast(uint32_t, ls) == 0) continue;  // a part without a visible key
-    const float ms = p.part_ml[slot * 2];
-    const floatx4 os = *(const floatx4*)(p.part_o + slot * kHeadDim + d);
-    const float mn = fmaxf(m, ms);
-    const float a = fast_exp2(m - mn), e = fast_exp2(ms - mn);
-    l = l * a + ls * e;
-    o = o * a + os * e;
-    m = mn;
+  float l = 0.f;
+  if (pos >= 0 && pos < row.len) {
+    int lo, hi;
+    row_positions(p, row, tile * p.tile_rows, (tile + 1) * p.tile_rows - 1, lo, hi);
+    const int n = span_of(p, row, lo, hi).n;
+    const int size = (n + s.parts - 1) / s.parts;
+    const int64_t step = (int64_t)rt.count * p.num_kv_heads * p.part_rows;
+    int64_t slot = ((int64_t)(s.before + rt.first + rt.count - 1 - tile) * p.num_kv_heads + kvh) * p.part_rows +
+                   kr - tile * p.tile_rows;
+    float m = kNegBig;
+    for (int at = 0; at < n; at += size, slot += step) {
+      const float ls = p.part_ml[slot * 2 + 1];
+      if (__builtin_bit_cast(uint32_t, ls) == 0) continue;  // a part without a visible key
+      const float ms = p.part_ml[slot * 2];
+      const floatx4 os = *(const floatx4*)(p.part_o + slot * kHeadDim + d);
+      const float mn = fmaxf(m, ms);
+      const float a = fast_exp2(m - mn), e = fast_exp2(ms - mn);
+      l = l * a + ls * e;
+      o = o * a + os * e;
+      m = mn;
+    }
   }
   const float inv = __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
   if (d < p.head_dim)
@@ -641,12 +734,13 @@ __global__ __launch_bounds__(32 * kMergeRows) void merge_kernel(Params p) {
         to_half4(o * inv);
 }
 
-// How a call is cut: row blocks per wave, row tiles per (row, kv head), parts per row tile.
-constexpr int64_t kSlots = 512;  // workgroups resident at once: two per CU
-constexpr int kMinPart = 4;
+// How a call is cut: row blocks per wave, row tiles per (batch row, kv head), list entries and
+// results' rows of the parts (0: not cut).
+constexpr int64_t kMaxWgs = (1 << 24) - 1;  // a launch takes fewer than 2^32 threads along x
 struct Plan {
   int nb;
-  int64_t row_tiles, splits;
+  int64_t row_tiles, wgs, target, part_rows;
+  size_t bytes() const { return (size_t)((target + wgs) * part_rows * (kHeadDim + 2)) * sizeof(float); }
 };
 static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads,
                  int64_t num_tokens) {
@@ -654,15 +748,10 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
   Plan pl;
   pl.nb = (int)std::min<int64_t>((rows + 63) / 64, kMaxNb);
   pl.row_tiles = (rows + 64 * pl.nb - 1) / (64 * pl.nb);
-  const int64_t wgs = batch * num_kv_heads * pl.row_tiles;
-  const int64_t tiles = (num_tokens + kKTile - 1) / kKTile;
-  pl.splits = std::max<int64_t>(std::min(kSlots / wgs, (tiles + kMinPart - 1) / kMinPart), 1);
+  pl.wgs = batch * num_kv_heads * pl.row_tiles;
+  pl.target = pl.wgs < kSlots && num_tokens > kMinPart * kKTile ? kSlots : 0;
+  pl.part_rows = pl.target ? std::min<int64_t>(rows, 64 * pl.nb) : 0;
   return pl;
-}
-
-// Bytes of `splits` parts a query row.
-static size_t part_bytes(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t splits) {
-  return splits <= 1 ? 0 : (size_t)(batch * chunk * num_q_heads * splits * (kHeadDim + 2)) * sizeof(float);
 }
 
 static bool sizes_ok(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads) {
@@ -692,8 +781,8 @@ extern "C" size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t
       max_num_tokens <= 0 || max_num_tokens > kMaxTokens || !fi::head_dim_ok(head_dim) ||
       batch > 0x7fffffff || num_new > 0x7fffffff / num_q_heads)
     return 0;
-  return part_bytes(batch, num_new, num_q_heads,
-                    plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens).splits);
+  const Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens);
+  return pl.target ? pl.bytes() : 0;
 }
 
 extern "C" int fi_paged_chunk_attention_fwd(
@@ -737,8 +826,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
   if (batch == 0 || num_new == 0) return FI_OK;
   if (num_tokens > kMaxTokens || num_pool_blocks > 0x7fffffff / block_size ||
       max_blocks_per_seq > 0x7fffffff || batch > 0x7fffffff / num_kv_heads ||
-      num_new > 0x7fffffff / num_q_heads / 2 ||
-      batch * num_new > (int64_t)0x7fffffff * kMergeRows / num_q_heads) {
+      num_new > 0x7fffffff / num_q_heads / 2) {
     set_error("%s: sizes too large (at most %lld tokens a row, 2^31 pool slots)", fn,
               (long long)kMaxTokens);
     return FI_ERR_UNSUPPORTED;
@@ -782,7 +870,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.d_chunks = (int)(head_dim / 8);
   if (softcap > 0.f) {
     p.scale_log2 = 1.f;
-    p.cap_arg = cap_arg;
+    p.cap_exp = cap_arg * (2.f * kLog2e);
     p.cap_log2 = softcap * kLog2e;
   } else {
     // scores are masked before they are scaled and -inf * 0 is NaN: a zero scale runs as unit
@@ -798,27 +886,28 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
   p.prefix_lens = prefix_lens;
 
-  const Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens);
-  const int64_t one = (int64_t)part_bytes(batch, num_new, num_q_heads, 2) / 2;
-  const int64_t room = workspace ? (int64_t)std::min<size_t>(workspace_bytes, (size_t)1 << 62) / one : 0;
-  const int64_t splits = std::min(pl.splits, std::max<int64_t>(room, 1));
-  p.rows_per_tile = 64 * pl.nb;
-  p.max_splits = (int)splits;
-  p.min_part = kMinPart;
-  const int64_t rows = batch * num_new * num_q_heads;
-  if (splits > 1) {
+  Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens);
+  if (pl.wgs > kMaxWgs) {
+    set_error("%s: too many new tokens (%lld rows of %lld)", fn, (long long)batch, (long long)num_new);
+    return FI_ERR_UNSUPPORTED;
+  }
+  if (pl.target && (!workspace || workspace_bytes < pl.bytes())) pl.target = 0;
+  p.tile_rows = 64 * pl.nb;
+  p.tile_div = fast_div((uint32_t)p.tile_rows);
+  p.row_tiles = (int)pl.row_tiles;
+  if (pl.target) {
     if ((uintptr_t)workspace & 15u) {
       set_error("%s: workspace must be 16-byte aligned", fn);
       return FI_ERR_INVALID;
     }
+    p.target = (int)pl.target;
+    p.part_rows = (int)pl.part_rows;
     p.part_o = (float*)workspace;
-    p.part_ml = p.part_o + rows * splits * kHeadDim;
+    p.part_ml = p.part_o + (pl.target + pl.wgs) * pl.part_rows * kHeadDim;
   }
-  if (pl.row_tiles > 65535) {
-    set_error("%s: too many new tokens (%lld)", fn, (long long)num_new);
-    return FI_ERR_UNSUPPORTED;
-  }
-  const dim3 grid((unsigned)(batch * num_kv_heads), (unsigned)pl.row_tiles, (unsigned)splits);
+  // list entries: at most target / num_kv_heads (rounded up) and one per row tile
+  const int64_t items = batch * pl.row_tiles + pl.target / num_kv_heads;
+  const dim3 grid((unsigned)(items * num_kv_heads));
   const hipStream_t st = (hipStream_t)stream;
   switch ((softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0)) {
     case 0: launch<0>(pl.nb, grid, st, p); break;
@@ -827,8 +916,9 @@ extern "C" int fi_paged_chunk_attention_fwd(
     default: launch<kCap | kBias>(pl.nb, grid, st, p); break;
   }
   const int rc = check_launch(fn);
-  if (rc != FI_OK || splits == 1) return rc;
-  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)((rows + kMergeRows - 1) / kMergeRows)),
-                     dim3(32 * kMergeRows), 0, st, p);
+  if (rc != FI_OK || !pl.target) return rc;
+  const int64_t merge_wgs = (num_new * num_q_heads + kMergeRows - 1) / kMergeRows;
+  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)merge_wgs, (unsigned)batch), dim3(32 * kMergeRows), 0, st,
+                     p);
   return check_launch(fn);
 }
