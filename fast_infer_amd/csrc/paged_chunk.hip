@@ -31,10 +31,7 @@ namespace chunk {
 
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
-constexpr int kKTile = 64;                      // keys per tile
-constexpr int kRowBytes = kHeadDim * 2;         // one K or V row in LDS
-constexpr int kTileBytes = kKTile * kRowBytes;  // 16 KiB
-constexpr int kStageBytes = 2 * kTileBytes;     // K + V
+constexpr int kKTile = 64;  // keys per tile
 constexpr int kMaxNb = 3;
 constexpr float kLazyLog2 = 8.f;  // the reference max may lag the true max by 2^8
 constexpr int kNoWindow = 0x3fffffff;
@@ -104,6 +101,7 @@ struct Params {
   int part_rows;      // min(tile_rows, chunk * group): rows of a part's results
   float* part_o;      // [parts, num_kv_heads][part_rows][128]; null: no parts, write o
   float* part_ml;     // [...][2]: reference max (log2 units), sum
+  int32_t* shares;    // [batch][2]: Share::before and parts, for the kernel that adds the parts
 };
 
 // What a batch row attends over.
@@ -183,8 +181,8 @@ __device__ __forceinline__ RowTiles row_tiles_of(const Params& p, const Row& row
 // key tiles to visit over the parts aimed at (kMinPart at least), each row tile of batch row b is
 // cut into parts(b) = ceil(its longest list / size) equal pieces, and the work list is, for each
 // b, its parts (row tile fastest, so that neighbours read the same keys), then its row tiles
-// without tokens, one each.  `size` and `before` (list entries of earlier batch rows) for row b;
-// with `item` >= 0, b is looked up from the list place.  Wave-wide; lanes hold batch rows.
+// without tokens, one each.  The batch row of list place `item` (-1 past the list), the
+// places before it and its parts.  Wave-wide; lanes hold batch rows.
 struct Share {
   int b, before, parts;
 };
@@ -193,7 +191,7 @@ __device__ __forceinline__ int wave_sum(int v) {
   for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
   return v;
 }
-__device__ __forceinline__ Share find_share(const Params& p, int item, int b, int lane) {
+__device__ __forceinline__ Share find_share(const Params& p, int item, int lane) {
   auto tiles_of = [&](int i) { return i < p.batch ? row_tiles_of(p, row_of(p, i)) : RowTiles{0, 0, 0}; };
   const RowTiles t0 = tiles_of(lane);
   int total = t0.count * t0.n;
@@ -216,9 +214,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int b, in
       if (lane >= d) upto += x;
     }
     upto += before;
-    const uint64_t hit =
-        item >= 0 ? __builtin_amdgcn_ballot_w64(upto > item) : (b >> 6) == (i0 >> 6) ? 1ull << (b & 63) : 0;
-    if (hit) {
+    if (const uint64_t hit = __builtin_amdgcn_ballot_w64(upto > item)) {
       const int l = __builtin_ctzll(hit);
       s.b = i0 + l;
       s.before = __builtin_amdgcn_readlane(upto - items, l);
@@ -230,14 +226,29 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int b, in
   return s;
 }
 
-// LDS tile layouts, as in the prefill kernel: a K tile is 4 panels of 64 bytes per key (chunks
-// XOR-permuted by (key >> 1) & 3, conflict-free fragment reads), a V tile 8 panels of 32 bytes
-// per key (conflict-free transpose reads).
-constexpr int kKPanel = kKTile * 64;
-constexpr int kVPanel = kKTile * 32;
+// LDS layout of a tile of kD-wide rows (64 or 128; a smaller head_dim leaves zeros).  Whole rows
+// of 2 kD bytes, as they lie in the pool, so that a copy instruction reads 1 KiB in full rows:
+// with 64- and 32-byte pieces of many rows (as the prefill kernel copies) long contexts streamed
+// at 3 TB/s.  The 16-byte chunks of a row are XOR-permuted: K fragment reads (16 rows, one chunk
+// per 16-lane group; the LDS serves 8 rows of two such groups at a time) and V transpose reads (8
+// rows, 32 bytes) are free of bank conflicts, and the fragments of a row differ by an XOR of the
+// address with a constant.
+template <int kD>
+struct Tile {
+  static constexpr int kRow = 2 * kD;           // bytes
+  static constexpr int kChunks = kD / 8;
+  static constexpr int kBytes = kKTile * kRow;  // of K or V
+  static constexpr int kStage = 2 * kBytes;
+  static constexpr int kCopyRows = 1024 / kRow;                // rows of one copy instruction
+  static constexpr int kCopies = kKTile / kWaves / kCopyRows;  // of a wave, each of K and V
+  static __device__ __forceinline__ int xk(int r) {
+    return (kD == 128 ? (r & 3) << 2 : (r & 2) << 1) | ((r >> 1) & 2);
+  }
+  static __device__ __forceinline__ int xv(int r) { return kD == 128 ? (r & 7) << 1 : r & 6; }
+};
 
-// The page that masked keys and the columns past head_dim are copied from.
-__device__ __attribute__((aligned(256))) const char g_zeros[kRowBytes] = {0};
+// The row that masked keys and the columns past head_dim are copied from.
+__device__ __attribute__((aligned(256))) const char g_zeros[2 * kHeadDim] = {0};
 
 // One direct-to-LDS copy from a 64-bit address per lane: 16 bytes to LDS byte lds + 16 * lane.
 // Through inline asm for the reasons given at lds_copy16; the callers wait for the copies
@@ -254,85 +265,100 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// This wave's eight copies (four of K, four of V) of the tile whose key `lane` lies in pool row
-// `row` (-1: zeros).  Wave w copies K keys 16w .. 16w + 15 and half the columns of V keys
-// 32 (w / 2) .. + 31.
+// This wave's copies (keys 16w .. 16w + 15, K and V) of the tile whose key `lane` lies in pool row
+// `row` (-1: zeros).
+template <int kD>
 __device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, const char* vbase,
                                            char* stage, int row, int w, int lane) {
-  const int rk = __shfl(row, 16 * w + (lane >> 2));
-  const int rv = __shfl(row, 32 * (w >> 1) + (lane >> 1));
-  const char* ks = rk >= 0 ? kbase + rk * p.row_bytes : g_zeros;
-  const char* vs = rv >= 0 ? vbase + rv * p.row_bytes : g_zeros;
-  const uint32_t kd = lds_addr(stage) + 16 * w * 64;
-  const uint32_t vd = lds_addr(stage) + kTileBytes + 32 * (w >> 1) * 32;
-  const int kc = (lane & 3) ^ ((lane >> 3) & 3);
+  typedef Tile<kD> T;
+  const int slot = lane % T::kChunks;
+  const uint32_t dst = lds_addr(stage) + 16 * w * T::kRow;
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int ch = 4 * q + kc;
-    lds_copy16_global(ch < p.d_chunks ? ks + 16 * ch : g_zeros, kd + q * kKPanel);
-    const int panel = 4 * (w & 1) + q;
-    const int vch = 2 * panel + (lane & 1);
-    lds_copy16_global(vch < p.d_chunks ? vs + 16 * vch : g_zeros, vd + panel * kVPanel);
+  for (int q = 0; q < T::kCopies; ++q) {
+    const int r = q * T::kCopyRows + lane / T::kChunks;
+    const int from = __shfl(row, 16 * w + r);
+    const int64_t at = from * p.row_bytes;
+    const int kc = slot ^ T::xk(r), vc = slot ^ T::xv(r);
+    lds_copy16_global((from >= 0 && kc < p.d_chunks ? kbase + at : g_zeros) + 16 * kc, dst + 1024 * q);
+    lds_copy16_global((from >= 0 && vc < p.d_chunks ? vbase + at : g_zeros) + 16 * vc,
+                      dst + T::kBytes + 1024 * q);
   }
 }
 
-// V^T fragment half: lane (col, g) receives keys row0 + 4g + j (j = 0..3) of column 16 dt + col.
-__device__ __forceinline__ u32x2 vt_read(const char* vs, int row0, int dt, int col, int g) {
-  typedef short s4 __attribute__((ext_vector_type(4)));
-  const char* ptr = vs + dt * kVPanel + (row0 + 4 * g + (col >> 2)) * 32 + ((col & 3) << 3);
-  const s4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4 __attribute__((address_space(3)))*)ptr);
-  return __builtin_bit_cast(u32x2, v);
+// V^T fragment of slice c: lane (col, g) receives keys 32c + 4g + j and 32c + 16 + 4g + j (j = 0..3)
+// of column 16 dt + col.  vs: the V tile at this lane's place for dt = 0 (v_lane).
+template <int kD>
+__device__ __forceinline__ int v_lane(int col, int g) {
+  const int r = 4 * g + (col >> 2);
+  return r * Tile<kD>::kRow + ((((col & 3) >> 1) ^ Tile<kD>::xv(r)) << 4) + ((col & 1) << 3);
 }
-__device__ __forceinline__ half8 vt_frag(const char* vs, int c, int dt, int col, int g) {
-  const u32x2 a0 = vt_read(vs, 32 * c, dt, col, g);
-  const u32x2 a1 = vt_read(vs, 32 * c + 16, dt, col, g);
+template <int kD>
+__device__ __forceinline__ half8 vt_frag(uint32_t vs, int c, int dt) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  typedef s4 __attribute__((address_space(3))) * lds_s4;
+  const uint32_t at = (vs ^ (dt << 5)) + 32 * c * Tile<kD>::kRow;
+  const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at);
+  const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 16 * Tile<kD>::kRow));
+  const u32x2 a0 = __builtin_bit_cast(u32x2, a), a1 = __builtin_bit_cast(u32x2, b);
   return as_half8(u32x4{a0[0], a0[1], a1[0], a1[1]});
 }
 
+// K fragment of slice c: lane (col, g) receives columns 32 i + 8 g .. + 7 of key 32c + 16t + col.
+template <int kD>
+__device__ __forceinline__ int k_lane(int col, int g) {
+  return col * Tile<kD>::kRow + ((g ^ Tile<kD>::xk(col)) << 4);
+}
+template <int kD>
+__device__ __forceinline__ half8 k_frag(uint32_t ks, int c, int t, int i) {
+  typedef u32x4 __attribute__((address_space(3))) * lds_u4;
+  return as_half8(*(lds_u4)((ks ^ (i << 6)) + (32 * c + 16 * t) * Tile<kD>::kRow));
+}
+
 // S^T = K Q^T + init for the 32-key slice c: s[j][t] holds keys 32c + 16t + 4g + r of row block j.
-template <int NB>
-__device__ __forceinline__ void qk_slice(const char* ks, int c, int col, int g,
-                                         const half8 (&qf)[NB][4], floatx4 (&s)[NB][2]) {
-  auto frag = [&](int u) {
-    const int t = u >> 2, i = u & 3;
-    return as_half8(*(const u32x4*)(ks + i * kKPanel + (32 * c + 16 * t + col) * 64 +
-                                    ((g ^ ((col >> 1) & 3)) << 4)));
-  };
-  half8 cur = frag(0);
+template <int NB, int kD>
+__device__ __forceinline__ void qk_slice(uint32_t ks, int c, const half8 (&qf)[NB][kD / 32],
+                                         floatx4 (&s)[NB][2]) {
+  constexpr int kI = kD / 32;
+  half8 cur = k_frag<kD>(ks, c, 0, 0);
 #pragma unroll
-  for (int u = 0; u < 8; ++u) {
+  for (int u = 0; u < 2 * kI; ++u) {
     half8 nxt;
-    if (u + 1 < 8) nxt = frag(u + 1);
+    if (u + 1 < 2 * kI) nxt = k_frag<kD>(ks, c, (u + 1) / kI, (u + 1) % kI);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) s[j][u >> 2] = mfma16x16x32(cur, qf[j][u & 3], s[j][u >> 2]);
-    if (u + 1 < 8) cur = nxt;
+    for (int j = 0; j < NB; ++j) s[j][u / kI] = mfma16x16x32(cur, qf[j][u % kI], s[j][u / kI]);
+    if (u + 1 < 2 * kI) cur = nxt;
   }
 }
 
-// O^T += V^T P^T of slice c (accumulator tiles 0..7) and the sums of P (tile 8, all-ones A).
-template <int NB>
-__device__ __forceinline__ void pv_slice(const char* vs, int c, int col, int g, const half8 (&pf)[NB],
-                                         floatx4 (&acc)[NB][9]) {
-  half8 vf = vt_frag(vs, c, 0, col, g);
+__device__ __forceinline__ half8 ones8() {
+  return as_half8(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
+}
+
+// O^T += V^T P^T of slice c, and the sums of P (last accumulator tile, all-ones A).
+template <int NB, int kD>
+__device__ __forceinline__ void pv_slice(uint32_t vs, int c, const half8 (&pf)[NB],
+                                         floatx4 (&acc)[NB][kD / 16 + 1]) {
+  constexpr int kT = kD / 16;
+  half8 vf = vt_frag<kD>(vs, c, 0);
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) {
+  for (int dt = 0; dt < kT; ++dt) {
     half8 vn;
-    if (dt + 1 < 8) vn = vt_frag(vs, c, dt + 1, col, g);
+    if (dt + 1 < kT) vn = vt_frag<kD>(vs, c, dt + 1);
 #pragma unroll
     for (int j = 0; j < NB; ++j) acc[j][dt] = mfma16x16x32(vf, pf[j], acc[j][dt]);
-    if (dt + 1 < 8) vf = vn;
+    if (dt + 1 < kT) vf = vn;
   }
-  const half8 ones = as_half8(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 #pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j][8] = mfma16x16x32(ones, pf[j], acc[j][8]);
+  for (int j = 0; j < NB; ++j) acc[j][kT] = mfma16x16x32(ones8(), pf[j], acc[j][kT]);
 }
 
 // Whether slice c of V is finite: the product with an all-zero P is NaN where V is not.
-__device__ __forceinline__ bool v_finite(const char* vs, int c, int col, int g) {
+template <int kD>
+__device__ __forceinline__ bool v_finite(uint32_t vs, int c) {
   const half8 zero = as_half8(u32x4{0u, 0u, 0u, 0u});
   floatx4 chk = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) chk = mfma16x16x32(vt_frag(vs, c, dt, col, g), zero, chk);
+  for (int dt = 0; dt < kD / 16; ++dt) chk = mfma16x16x32(vt_frag<kD>(vs, c, dt), zero, chk);
   // the file is compiled for NaN-free arithmetic: hide where the bits are from
   asm volatile("" : "+v"(chk));
   const u32x4 u = __builtin_bit_cast(u32x4, chk);
@@ -344,13 +370,14 @@ __device__ __forceinline__ bool v_finite(const char* vs, int c, int col, int g) 
 // in the matrix product would reach those rows.  The product runs on V with such values
 // replaced by zeros; then products of indicators (V is +inf or NaN / -inf or NaN; P is not zero)
 // count which of them each row sees, and put the infinities where they belong (both: NaN).
-template <int NB>
-__device__ __forceinline__ void pv_slice_careful(const char* vs, int c, int col, int g,
-                                                 const half8 (&pf)[NB], floatx4 (&acc)[NB][9]) {
+template <int NB, int kD>
+__device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c, const half8 (&pf)[NB],
+                                                 floatx4 (&acc)[NB][kD / 16 + 1]) {
   typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+  constexpr int kT = kD / 16;
 #pragma unroll
-  for (int dt = 0; dt < 8; ++dt) {
-    const us8 v = __builtin_bit_cast(us8, vt_frag(vs, c, dt, col, g));
+  for (int dt = 0; dt < kT; ++dt) {
+    const us8 v = __builtin_bit_cast(us8, vt_frag<kD>(vs, c, dt));
     us8 ok, inf[2];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -378,9 +405,8 @@ __device__ __forceinline__ void pv_slice_careful(const char* vs, int c, int col,
       }
     }
   }
-  const half8 ones = as_half8(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 #pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j][8] = mfma16x16x32(ones, pf[j], acc[j][8]);
+  for (int j = 0; j < NB; ++j) acc[j][kT] = mfma16x16x32(ones8(), pf[j], acc[j][kT]);
 }
 
 // x = cap_log2 * tanh(y), y = s * sm_scale / cap, in log2 units: tanh(y) = 1 - 2 / (1 + e^2y).
@@ -402,14 +428,11 @@ __device__ __forceinline__ float capped_series(const Params& p, float s) {
 // One resident tile (keys k0 .. k0 + 63) for this wave's rows.  s_pos, s_slope: of the wave's rows;
 // keys: bit k is set when key k0 + k is before the row's length and in the pool; kMasked: some
 // row may not see some key.
-template <int NB, int kMod, bool kMasked>
-__device__ __forceinline__ void consume(const Params& p, const char* stage, int k0, uint64_t keys,
-                                        int prefix, const int* s_pos,
-                                        const float* s_slope, int col, int g,
-                                        const half8 (&qf)[NB][4], float (&t_run)[NB],
-                                        floatx4 (&acc)[NB][9]) {
-  const char* ks = stage;
-  const char* vs = stage + kTileBytes;
+template <int NB, int kD, int kMod, bool kMasked>
+__device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t vs, int k0, uint64_t keys,
+                                        int prefix, const int* s_pos, const float* s_slope, int col,
+                                        int g, const half8 (&qf)[NB][kD / 32], float (&t_run)[NB],
+                                        floatx4 (&acc)[NB][kD / 16 + 1]) {
 #pragma unroll
   for (int c = 0; c < kKTile / 32; ++c) {
     // a uniform branch, never taken, between the slices: without it the compiler overlaps the
@@ -426,7 +449,7 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
       for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[j][t][r] = kMod == kBias ? bias(j, t, r) : 0.f;
-    qk_slice<NB>(ks, c, col, g, qf, s);
+    qk_slice<NB, kD>(ks, c, qf, s);
     if (kMod & kCap) {
       const bool series = p.cap_log2 > kExpCap * kLog2e;
 #pragma unroll
@@ -487,7 +510,7 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
         const float alpha = fast_exp2((t_old - t_new) * p.scale_log2);
         t_run[j] = t_new;
 #pragma unroll
-        for (int dt = 0; dt < 9; ++dt) acc[j][dt] *= alpha;
+        for (int dt = 0; dt <= kD / 16; ++dt) acc[j][dt] *= alpha;
       }
     }
     // P is rounded to fp16 for the matrix cores; the sums take the rounded values too.
@@ -501,18 +524,19 @@ __device__ __forceinline__ void consume(const Params& p, const char* stage, int 
         for (int r = 0; r < 4; ++r)
           pf[j][4 * t + r] = (half_t)fast_exp2(__builtin_fmaf(s[j][t][r], p.scale_log2, -mc));
     }
-    if (kMasked && !v_finite(vs, c, col, g))
-      pv_slice_careful<NB>(vs, c, col, g, pf, acc);
+    if (kMasked && !v_finite<kD>(vs, c))
+      pv_slice_careful<NB, kD>(vs, c, pf, acc);
     else
-      pv_slice<NB>(vs, c, col, g, pf, acc);
+      pv_slice<NB, kD>(vs, c, pf, acc);
   }
 }
 
-template <int NB, int kMod>
+template <int NB, int kD, int kMod>
 __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
+  typedef Tile<kD> T;
   constexpr int kRowsPerWave = 16 * NB;
   constexpr int kRows = kWaves * kRowsPerWave;
-  __shared__ __attribute__((aligned(16))) char stages[2 * kStageBytes];
+  __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
   __shared__ int s_pos[kRows];      // position of each query row, -1 for rows without a token
   __shared__ float s_slope[kRows];  // its distance bias in score units
 
@@ -525,11 +549,12 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const int item = blockIdx.x / p.num_kv_heads;
   int b, tile, part = 0, parts = 1;
   if (p.part_o) {
-    const Share s = find_share(p, item, 0, lane);
+    const Share s = find_share(p, item, lane);
     if (s.b < 0) return;  // past the list
     b = s.b;
     const RowTiles rt = row_tiles_of(p, row_of(p, b));
     int at = item - s.before;
+    if (at == 0 && kvh == 0 && tid < 2) p.shares[2 * b + tid] = tid ? s.parts : s.before;
     if (at < rt.count * s.parts) {
       part = at / rt.count;
       parts = s.parts;
@@ -569,15 +594,15 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
 
   int row_next = pool_row(0, entry_of(0));
-  issue_tile(p, kbase, vbase, stages, row_next, w, lane);
+  issue_tile<kD>(p, kbase, vbase, stages, row_next, w, lane);
   uint64_t keys = __builtin_amdgcn_ballot_w64(row_next >= 0), keys_next = 0;
   row_next = pool_row(1, entry_of(1));
   keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
-  issue_tile(p, kbase, vbase, stages + kStageBytes, row_next, w, lane);
+  issue_tile<kD>(p, kbase, vbase, stages + T::kStage, row_next, w, lane);
   int entry = entry_of(2);
 
   // Q^T fragments: MFMA i takes d = 32 i + 8 g + s in reduction slot 8 g + s.
-  half8 qf[NB][4];
+  half8 qf[NB][kD / 32];
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     const int r = r0 + kRowsPerWave * w + 16 * j + col;
@@ -587,7 +612,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     const bool ok = t < p.chunk && pos >= 0 && pos < row.len;
     const half_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)(ok ? t : 0) * p.q_st + (int64_t)h * p.q_sh;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < kD / 32; ++i) {
       u32x4 v = {0u, 0u, 0u, 0u};
       if (ok && !p.q_zero && 32 * i + 8 * g < p.head_dim) v = *(const u32x4*)(src + 32 * i + 8 * g);
       qf[j][i] = as_half8(v ^ p.q_sign);
@@ -603,12 +628,12 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   row_positions(p, row, r0 + kRowsPerWave * w, r0 + kRowsPerWave * (w + 1) - 1, wlo, whi);
 
   float t_run[NB];
-  floatx4 acc[NB][9];  // O^T columns 16dt .. 16dt + 15 (dt < 8), sum of P (dt = 8)
+  floatx4 acc[NB][kD / 16 + 1];  // O^T columns 16dt .. 16dt + 15, then the sum of P
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
     t_run[j] = kNegBig;
 #pragma unroll
-    for (int dt = 0; dt < 9; ++dt) acc[j][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+    for (int dt = 0; dt <= kD / 16; ++dt) acc[j][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
   stage_barrier();
 
@@ -619,23 +644,26 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     row_next = pool_row(i + 1, entry);
     keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
     entry = entry_of(i + 2);
-    issue_tile(p, kbase, vbase, stages + ((i + 1) & 1) * kStageBytes, row_next, w, lane);
+    issue_tile<kD>(p, kbase, vbase, stages + ((i + 1) & 1) * T::kStage, row_next, w, lane);
   };
+  const uint32_t ks = lds_addr(stages) + k_lane<kD>(col, g);
+  const uint32_t vs = lds_addr(stages) + T::kBytes + v_lane<kD>(col, g);
   int i = 0;
   for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
     copy_next(i);
     const int k0 = span.tile(first + i) * kKTile;
     if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
-      consume<NB, kMod, true>(p, stages + (i & 1) * kStageBytes, k0, keys, row.prefix, w_pos, w_slope, col,
-                              g, qf, t_run, acc);
+      consume<NB, kD, kMod, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
+                                  row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
     keys = keys_next;
     stage_barrier();
   }
   for (; i < n; ++i) {
     copy_next(i);
     if (wlo <= whi)
-      consume<NB, kMod, false>(p, stages + (i & 1) * kStageBytes, span.tile(first + i) * kKTile, keys,
-                               row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
+      consume<NB, kD, kMod, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
+                                   span.tile(first + i) * kKTile, keys, row.prefix, w_pos, w_slope, col, g,
+                                   qf, t_run, acc);
     keys = keys_next;
     stage_barrier();
   }
@@ -647,54 +675,56 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
       if (w_pos[16 * j + col] < 0) continue;
       const int64_t slot = (int64_t)blockIdx.x * p.part_rows + rl;
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
-        *(floatx4*)(p.part_o + slot * kHeadDim + 16 * dt + 4 * g) = acc[j][dt];
+      for (int dt = 0; dt < kD / 16; ++dt) *(floatx4*)(p.part_o + slot * kD + 16 * dt + 4 * g) = acc[j][dt];
       if (g == 0) {
         p.part_ml[slot * 2] = __builtin_fmaf(t_run[j], p.scale_log2, -p.lazy_log2);
-        p.part_ml[slot * 2 + 1] = acc[j][8][0];
+        p.part_ml[slot * 2 + 1] = acc[j][kD / 16][0];
       }
     }
     return;
   }
 
   // Normalise; the rows go through this wave's part of the stages (idle since the last barrier)
-  // so that each store instruction writes whole rows.  Rows are padded to 272 bytes: the 16
-  // rows of one write land in distinct banks.
-  constexpr int kORow = 272;
-  static_assert(kWaves * kRowsPerWave * kORow <= 2 * kStageBytes, "output rows fit the stages");
+  // so that each store instruction writes whole rows.  Rows are padded by 16 bytes: the 16 rows of
+  // one write land in distinct banks.
+  constexpr int kORow = T::kRow + 16;
+  static_assert(kWaves * kRowsPerWave * kORow <= 2 * T::kStage, "output rows fit the stages");
   char* ostage = stages + w * kRowsPerWave * kORow;
 #pragma unroll
   for (int j = 0; j < NB; ++j) {
-    const float l = acc[j][8][0];
+    const float l = acc[j][kD / 16][0];
     const float inv = w_pos[16 * j + col] >= 0 && __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
     char* orow = ostage + (16 * j + col) * kORow + 8 * g;
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) *(half4*)(orow + 32 * dt) = to_half4(acc[j][dt] * inv);
+    for (int dt = 0; dt < kD / 16; ++dt) *(half4*)(orow + 32 * dt) = to_half4(acc[j][dt] * inv);
   }
   wave_lds_sync();
-  const int r4 = lane >> 4, c16 = lane & 15;
+  const int orl = lane / T::kChunks, oc = lane % T::kChunks;
 #pragma unroll
-  for (int rr = 0; rr < kRowsPerWave / 4; ++rr) {
-    const int rl = 4 * rr + r4;
+  for (int rr = 0; rr < kRowsPerWave / T::kCopyRows; ++rr) {
+    const int rl = T::kCopyRows * rr + orl;
     const int r = r0 + kRowsPerWave * w + rl;
     const int t = div_by(r, p.group_div);
     const int h = kvh * p.group + r - t * p.group;
-    const u32x4 v = *(const u32x4*)(ostage + rl * kORow + 16 * c16);
-    if (t < p.chunk && c16 < p.d_chunks)
-      *(u32x4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * c16) = v;
+    const u32x4 v = *(const u32x4*)(ostage + rl * kORow + 16 * oc);
+    if (t < p.chunk && oc < p.d_chunks)
+      *(u32x4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * oc) = v;
   }
 }
 
-// Adds the parts of each query row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  32 lanes a
-// row, four columns a lane; grid (rows of a batch row, batch).  Batch rows that were not cut, and
-// rows without a token, were written by the kernel above.
-constexpr int kMergeRows = 8;
-__global__ __launch_bounds__(32 * kMergeRows) void merge_kernel(Params p) {
+// Adds the parts of each query row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  Four
+// columns a lane; grid (rows of a batch row, batch).  Batch rows that were not cut, and row tiles
+// without a token, were written by the kernel above.  All loads of kMergeParts parts are issued at once.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeParts = 8;
+template <int kD>
+__global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
+  constexpr int kLanes = kD / 4;  // of a row
   const int b = blockIdx.y;
-  const Share s = find_share(p, -1, b, threadIdx.x & 63);
-  if (s.parts <= 1) return;
-  const int r = blockIdx.x * kMergeRows + (threadIdx.x >> 5);  // (token, query head)
-  const int d = 4 * (threadIdx.x & 31);
+  const int before = p.shares[2 * b], parts = p.shares[2 * b + 1];
+  if (parts <= 1) return;
+  const int r = blockIdx.x * (kMergeThreads / kLanes) + threadIdx.x / kLanes;  // (token, query head)
+  const int d = 4 * (threadIdx.x % kLanes);
   if (r >= p.chunk * p.num_q_heads) return;
   const int t = r / p.num_q_heads;
   const int h = r - t * p.num_q_heads;
@@ -706,26 +736,37 @@ __global__ __launch_bounds__(32 * kMergeRows) void merge_kernel(Params p) {
   const int tile = div_by(kr, p.tile_div);
   if (tile < rt.first || tile >= rt.first + rt.count) return;
   floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
+  float m = kNegBig, l = 0.f;
   if (pos >= 0 && pos < row.len) {
     int lo, hi;
     row_positions(p, row, tile * p.tile_rows, (tile + 1) * p.tile_rows - 1, lo, hi);
     const int n = span_of(p, row, lo, hi).n;
-    const int size = (n + s.parts - 1) / s.parts;
+    const int size = (n + parts - 1) / parts;
+    const int used = (n + size - 1) / size;  // parts with key tiles
     const int64_t step = (int64_t)rt.count * p.num_kv_heads * p.part_rows;
-    int64_t slot = ((int64_t)(s.before + rt.first + rt.count - 1 - tile) * p.num_kv_heads + kvh) * p.part_rows +
-                   kr - tile * p.tile_rows;
-    float m = kNegBig;
-    for (int at = 0; at < n; at += size, slot += step) {
-      const float ls = p.part_ml[slot * 2 + 1];
-      if (__builtin_bit_cast(uint32_t, ls) == 0) continue;  // a part without a visible key
-      const float ms = p.part_ml[slot * 2];
-      const floatx4 os = *(const floatx4*)(p.part_o + slot * kHeadDim + d);
-      const float mn = fmaxf(m, ms);
-      const float a = fast_exp2(m - mn), e = fast_exp2(ms - mn);
-      l = l * a + ls * e;
-      o = o * a + os * e;
-      m = mn;
+    const int64_t slot0 = ((int64_t)(before + rt.first + rt.count - 1 - tile) * p.num_kv_heads + kvh) *
+                              p.part_rows + kr - tile * p.tile_rows;
+    for (int s0 = 0; s0 < used; s0 += kMergeParts) {
+      float ms[kMergeParts], ls[kMergeParts];
+      floatx4 os[kMergeParts];
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        const int64_t slot = slot0 + min(s0 + k, used - 1) * step;
+        ms[k] = p.part_ml[slot * 2];
+        ls[k] = p.part_ml[slot * 2 + 1];
+        os[k] = *(const floatx4*)(p.part_o + slot * kD + d);
+      }
+#pragma unroll
+      for (int k = 0; k < kMergeParts; ++k) {
+        // (a part without a visible key has l = 0; a NaN is not)
+        const bool use = s0 + k < used && __builtin_bit_cast(uint32_t, ls[k]) != 0;
+        const float mn = fmaxf(m, use ? ms[k] : kNegBig);
+        const float a = fast_exp2(m - mn), e = use ? fast_exp2(ms[k] - mn) : 0.f;
+        l = l * a + (use ? ls[k] : 0.f) * e;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[c] = o[c] * a + (use ? os[k][c] : 0.f) * e;
+        m = mn;
+      }
     }
   }
   const float inv = __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
@@ -739,13 +780,16 @@ __global__ __launch_bounds__(32 * kMergeRows) void merge_kernel(Params p) {
 constexpr int64_t kMaxWgs = (1 << 24) - 1;  // a launch takes fewer than 2^32 threads along x
 struct Plan {
   int nb;
-  int64_t row_tiles, wgs, target, part_rows;
-  size_t bytes() const { return (size_t)((target + wgs) * part_rows * (kHeadDim + 2)) * sizeof(float); }
+  int64_t row_tiles, wgs, target, part_rows, width;
+  size_t bytes(int64_t batch) const {
+    return (size_t)((target + wgs) * part_rows * (width + 2) + 2 * batch) * sizeof(float);
+  }
 };
 static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads,
-                 int64_t num_tokens) {
+                 int64_t num_tokens, int64_t head_dim) {
   const int64_t rows = chunk * (num_q_heads / num_kv_heads);
   Plan pl;
+  pl.width = head_dim <= 64 ? 64 : 128;
   pl.nb = (int)std::min<int64_t>((rows + 63) / 64, kMaxNb);
   pl.row_tiles = (rows + 64 * pl.nb - 1) / (64 * pl.nb);
   pl.wgs = batch * num_kv_heads * pl.row_tiles;
@@ -759,15 +803,24 @@ static bool sizes_ok(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t 
          num_q_heads % num_kv_heads == 0;
 }
 
-template <int kMod>
+template <int kD, int kMod>
 static void launch(int nb, dim3 grid, hipStream_t st, const Params& p) {
   const dim3 block(kThreads);
   if (nb == 1)
-    hipLaunchKernelGGL((chunk_kernel<1, kMod>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((chunk_kernel<1, kD, kMod>), grid, block, 0, st, p);
   else if (nb == 2)
-    hipLaunchKernelGGL((chunk_kernel<2, kMod>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((chunk_kernel<2, kD, kMod>), grid, block, 0, st, p);
   else
-    hipLaunchKernelGGL((chunk_kernel<3, kMod>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((chunk_kernel<3, kD, kMod>), grid, block, 0, st, p);
+}
+template <int kD>
+static void launch(int mod, int nb, dim3 grid, hipStream_t st, const Params& p) {
+  switch (mod) {
+    case 0: launch<kD, 0>(nb, grid, st, p); break;
+    case kCap: launch<kD, kCap>(nb, grid, st, p); break;
+    case kBias: launch<kD, kBias>(nb, grid, st, p); break;
+    default: launch<kD, kCap | kBias>(nb, grid, st, p); break;
+  }
 }
 
 }  // namespace chunk
@@ -781,8 +834,8 @@ extern "C" size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t
       max_num_tokens <= 0 || max_num_tokens > kMaxTokens || !fi::head_dim_ok(head_dim) ||
       batch > 0x7fffffff || num_new > 0x7fffffff / num_q_heads)
     return 0;
-  const Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens);
-  return pl.target ? pl.bytes() : 0;
+  const Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens, head_dim);
+  return pl.target ? pl.bytes(batch) : 0;
 }
 
 extern "C" int fi_paged_chunk_attention_fwd(
@@ -886,12 +939,12 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
   p.prefix_lens = prefix_lens;
 
-  Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens);
+  Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens, head_dim);
   if (pl.wgs > kMaxWgs) {
     set_error("%s: too many new tokens (%lld rows of %lld)", fn, (long long)batch, (long long)num_new);
     return FI_ERR_UNSUPPORTED;
   }
-  if (pl.target && (!workspace || workspace_bytes < pl.bytes())) pl.target = 0;
+  if (pl.target && (!workspace || workspace_bytes < pl.bytes(batch))) pl.target = 0;
   p.tile_rows = 64 * pl.nb;
   p.tile_div = fast_div((uint32_t)p.tile_rows);
   p.row_tiles = (int)pl.row_tiles;
@@ -903,22 +956,25 @@ extern "C" int fi_paged_chunk_attention_fwd(
     p.target = (int)pl.target;
     p.part_rows = (int)pl.part_rows;
     p.part_o = (float*)workspace;
-    p.part_ml = p.part_o + (pl.target + pl.wgs) * pl.part_rows * kHeadDim;
+    p.part_ml = p.part_o + (pl.target + pl.wgs) * pl.part_rows * pl.width;
+    p.shares = (int32_t*)(p.part_ml + (pl.target + pl.wgs) * pl.part_rows * 2);
   }
   // list entries: at most target / num_kv_heads (rounded up) and one per row tile
   const int64_t items = batch * pl.row_tiles + pl.target / num_kv_heads;
   const dim3 grid((unsigned)(items * num_kv_heads));
   const hipStream_t st = (hipStream_t)stream;
-  switch ((softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0)) {
-    case 0: launch<0>(pl.nb, grid, st, p); break;
-    case kCap: launch<kCap>(pl.nb, grid, st, p); break;
-    case kBias: launch<kBias>(pl.nb, grid, st, p); break;
-    default: launch<kCap | kBias>(pl.nb, grid, st, p); break;
-  }
+  const int mod = (softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0);
+  if (pl.width == 64)
+    launch<64>(mod, pl.nb, grid, st, p);
+  else
+    launch<128>(mod, pl.nb, grid, st, p);
   const int rc = check_launch(fn);
   if (rc != FI_OK || !pl.target) return rc;
-  const int64_t merge_wgs = (num_new * num_q_heads + kMergeRows - 1) / kMergeRows;
-  hipLaunchKernelGGL(merge_kernel, dim3((unsigned)merge_wgs, (unsigned)batch), dim3(32 * kMergeRows), 0, st,
-                     p);
+  const int64_t merge_rows = kMergeThreads / (pl.width / 4);
+  const dim3 mgrid((unsigned)((num_new * num_q_heads + merge_rows - 1) / merge_rows), (unsigned)batch);
+  if (pl.width == 64)
+    hipLaunchKernelGGL(merge_kernel<64>, mgrid, dim3(kMergeThreads), 0, st, p);
+  else
+    hipLaunchKernelGGL(merge_kernel<128>, mgrid, dim3(kMergeThreads), 0, st, p);
   return check_launch(fn);
 }
