@@ -32,12 +32,10 @@ namespace chunk {
 constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kKTile = 64;  // keys per tile
-constexpr int kMaxNb = 3;
 constexpr float kLazyLog2 = 8.f;  // the reference max may lag the true max by 2^8
 constexpr int kNoWindow = 0x3fffffff;
 constexpr int64_t kMaxTokens = (int64_t)1 << 22;
-constexpr int kMinPart = 2;      // key tiles of the smallest part
-constexpr int64_t kSlots = 512;  // workgroups resident at once (two per CU): parts aimed at
+constexpr int kMinPart = 2;  // key tiles of the smallest part
 // Largest cap whose tanh is taken from exp2 alone: its absolute error, about 2e-7, times the
 // cap is an error of the logit, here 1e-4.
 constexpr float kExpCap = 500.f;
@@ -249,6 +247,8 @@ struct Tile {
 
 // The row that masked keys and the columns past head_dim are copied from.
 __device__ __attribute__((aligned(256))) const char g_zeros[2 * kHeadDim] = {0};
+// The table entry of keys that are not to be read.
+__device__ const int32_t g_no_block = -1;
 
 // One direct-to-LDS copy from a 64-bit address per lane: 16 bytes to LDS byte lds + 16 * lane.
 // Through inline asm for the reasons given at lds_copy16; the callers wait for the copies
@@ -260,23 +260,36 @@ __device__ __forceinline__ void lds_copy16_global(const char* src, uint32_t lds)
                : "memory");
 }
 
+// The same with 4 bytes a lane.
+__device__ __forceinline__ void lds_copy4_global(const int32_t* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
+               :
+               : "s"(lds), "v"(src)
+               : "memory");
+}
+// All but the last N of this wave's copies have landed (they do in order).
+template <int N>
+__device__ __forceinline__ void wait_copies() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 // This wave's copies have landed, its LDS reads are done, and every other wave says the same.
 __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// This wave's copies (keys 16w .. 16w + 15, K and V) of the tile whose key `lane` lies in pool row
-// `row` (-1: zeros).
+// This wave's copies of a tile: K and V of keys 16w .. 16w + 15, whose pool rows (-1: zeros) lanes
+// lane0 .. lane0 + 15 hold in `row`.
 template <int kD>
 __device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, const char* vbase,
-                                           char* stage, int row, int w, int lane) {
+                                           char* stage, int row, int lane0, int w, int lane) {
   typedef Tile<kD> T;
   const int slot = lane % T::kChunks;
   const uint32_t dst = lds_addr(stage) + 16 * w * T::kRow;
 #pragma unroll
   for (int q = 0; q < T::kCopies; ++q) {
     const int r = q * T::kCopyRows + lane / T::kChunks;
-    const int from = __shfl(row, 16 * w + r);
+    const int from = __shfl(row, lane0 + r);
     const int64_t at = from * p.row_bytes;
     const int kc = slot ^ T::xk(r), vc = slot ^ T::xv(r);
     lds_copy16_global((from >= 0 && kc < p.d_chunks ? kbase + at : g_zeros) + 16 * kc, dst + 1024 * q);
@@ -285,80 +298,124 @@ __device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, c
   }
 }
 
-// V^T fragment of slice c: lane (col, g) receives keys 32c + 4g + j and 32c + 16 + 4g + j (j = 0..3)
-// of column 16 dt + col.  vs: the V tile at this lane's place for dt = 0 (v_lane).
+// A slice of 16 kT keys (kT = 2 or 1) is what one step of the softmax covers.  P and V^T fragments
+// hold 4 kT keys a lane: with kT = 2 keys 4g + j and 16 + 4g + j (j = 0..3) in slots j and 4 + j.
+template <int kT>
+struct Slice;
+template <>
+struct Slice<2> {
+  typedef half8 frag;
+  typedef unsigned short bits __attribute__((ext_vector_type(8)));
+  static __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return mfma16x16x32(a, b, c); }
+};
+template <>
+struct Slice<1> {
+  typedef half4 frag;
+  typedef unsigned short bits __attribute__((ext_vector_type(4)));
+  static __device__ __forceinline__ floatx4 mfma(half4 a, half4 b, floatx4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
+  }
+};
+template <int kT>
+__device__ __forceinline__ typename Slice<kT>::frag splat(float x) {
+  typename Slice<kT>::frag f;
+#pragma unroll
+  for (int e = 0; e < 4 * kT; ++e) f[e] = (half_t)x;
+  return f;
+}
+
+// V^T fragment of slice c: lane (col, g) receives its keys of column 16 dt + col.  vs: LDS address
+// of the V tile at this lane's place for dt = 0 (v_lane).
 template <int kD>
 __device__ __forceinline__ int v_lane(int col, int g) {
   const int r = 4 * g + (col >> 2);
   return r * Tile<kD>::kRow + ((((col & 3) >> 1) ^ Tile<kD>::xv(r)) << 4) + ((col & 1) << 3);
 }
-template <int kD>
-__device__ __forceinline__ half8 vt_frag(uint32_t vs, int c, int dt) {
+template <int kD, int kT>
+__device__ __forceinline__ typename Slice<kT>::frag vt_frag(uint32_t vs, int c, int dt) {
   typedef short s4 __attribute__((ext_vector_type(4)));
   typedef s4 __attribute__((address_space(3))) * lds_s4;
-  const uint32_t at = (vs ^ (dt << 5)) + 32 * c * Tile<kD>::kRow;
-  const s4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at);
-  const s4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 16 * Tile<kD>::kRow));
-  const u32x2 a0 = __builtin_bit_cast(u32x2, a), a1 = __builtin_bit_cast(u32x2, b);
-  return as_half8(u32x4{a0[0], a0[1], a1[0], a1[1]});
+  const uint32_t at = (vs ^ (dt << 5)) + 16 * kT * c * Tile<kD>::kRow;
+  const half4 a = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at));
+  if constexpr (kT == 1) {
+    return a;
+  } else {
+    const half4 b = __builtin_bit_cast(
+        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 16 * Tile<kD>::kRow)));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  }
 }
 
-// K fragment of slice c: lane (col, g) receives columns 32 i + 8 g .. + 7 of key 32c + 16t + col.
+// K fragment: lane (col, g) receives columns 32 i + 8 g .. + 7 of key 16 kt + col.
 template <int kD>
 __device__ __forceinline__ int k_lane(int col, int g) {
   return col * Tile<kD>::kRow + ((g ^ Tile<kD>::xk(col)) << 4);
 }
 template <int kD>
-__device__ __forceinline__ half8 k_frag(uint32_t ks, int c, int t, int i) {
+__device__ __forceinline__ half8 k_frag(uint32_t ks, int kt, int i) {
   typedef u32x4 __attribute__((address_space(3))) * lds_u4;
-  return as_half8(*(lds_u4)((ks ^ (i << 6)) + (32 * c + 16 * t) * Tile<kD>::kRow));
+  return as_half8(*(lds_u4)((ks ^ (i << 6)) + 16 * kt * Tile<kD>::kRow));
 }
 
-// S^T = K Q^T + init for the 32-key slice c: s[j][t] holds keys 32c + 16t + 4g + r of row block j.
-template <int NB, int kD>
+// S^T = K Q^T + init for slice c: s[j][t] holds keys 16 (kT c + t) + 4g + r of row block j.  With one
+// row block a fragment feeds one product only, and waiting for each read in turn is what a slice
+// takes: all reads go first.  With more, one step ahead.
+template <int NB, int kD, int kT>
 __device__ __forceinline__ void qk_slice(uint32_t ks, int c, const half8 (&qf)[NB][kD / 32],
-                                         floatx4 (&s)[NB][2]) {
-  constexpr int kI = kD / 32;
-  half8 cur = k_frag<kD>(ks, c, 0, 0);
+                                         floatx4 (&s)[NB][kT]) {
+  constexpr int kI = kD / 32, kN = kT * kI;
+  if constexpr (NB == 1) {
+    half8 f[kN];
 #pragma unroll
-  for (int u = 0; u < 2 * kI; ++u) {
-    half8 nxt;
-    if (u + 1 < 2 * kI) nxt = k_frag<kD>(ks, c, (u + 1) / kI, (u + 1) % kI);
+    for (int u = 0; u < kN; ++u) f[u] = k_frag<kD>(ks, kT * c + u / kI, u % kI);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) s[j][u / kI] = mfma16x16x32(cur, qf[j][u % kI], s[j][u / kI]);
-    if (u + 1 < 2 * kI) cur = nxt;
+    for (int u = 0; u < kN; ++u) s[0][u / kI] = mfma16x16x32(f[u], qf[0][u % kI], s[0][u / kI]);
+  } else {
+    half8 cur = k_frag<kD>(ks, kT * c, 0);
+#pragma unroll
+    for (int u = 0; u < kN; ++u) {
+      half8 nxt;
+      if (u + 1 < kN) nxt = k_frag<kD>(ks, kT * c + (u + 1) / kI, (u + 1) % kI);
+#pragma unroll
+      for (int j = 0; j < NB; ++j) s[j][u / kI] = mfma16x16x32(cur, qf[j][u % kI], s[j][u / kI]);
+      if (u + 1 < kN) cur = nxt;
+    }
   }
-}
-
-__device__ __forceinline__ half8 ones8() {
-  return as_half8(u32x4{0x3C003C00u, 0x3C003C00u, 0x3C003C00u, 0x3C003C00u});
 }
 
 // O^T += V^T P^T of slice c, and the sums of P (last accumulator tile, all-ones A).
-template <int NB, int kD>
-__device__ __forceinline__ void pv_slice(uint32_t vs, int c, const half8 (&pf)[NB],
+template <int NB, int kD, int kT>
+__device__ __forceinline__ void pv_slice(uint32_t vs, int c, const typename Slice<kT>::frag (&pf)[NB],
                                          floatx4 (&acc)[NB][kD / 16 + 1]) {
-  constexpr int kT = kD / 16;
-  half8 vf = vt_frag<kD>(vs, c, 0);
+  constexpr int kN = kD / 16;
+  typename Slice<kT>::frag vf = vt_frag<kD, kT>(vs, c, 0);
 #pragma unroll
-  for (int dt = 0; dt < kT; ++dt) {
-    half8 vn;
-    if (dt + 1 < kT) vn = vt_frag<kD>(vs, c, dt + 1);
+  for (int dt = 0; dt < kN; ++dt) {
+    typename Slice<kT>::frag vn;
+    if (dt + 1 < kN) vn = vt_frag<kD, kT>(vs, c, dt + 1);
 #pragma unroll
-    for (int j = 0; j < NB; ++j) acc[j][dt] = mfma16x16x32(vf, pf[j], acc[j][dt]);
-    if (dt + 1 < kT) vf = vn;
+    for (int j = 0; j < NB; ++j) acc[j][dt] = Slice<kT>::mfma(vf, pf[j], acc[j][dt]);
+    if (dt + 1 < kN) vf = vn;
   }
 #pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j][kT] = mfma16x16x32(ones8(), pf[j], acc[j][kT]);
+  for (int j = 0; j < NB; ++j) acc[j][kN] = Slice<kT>::mfma(splat<kT>(1.f), pf[j], acc[j][kN]);
+}
+// The same for one row block, from fragments read before the softmax.
+template <int kD, int kT>
+__device__ __forceinline__ void pv_read(const typename Slice<kT>::frag (&vf)[kD / 16],
+                                        typename Slice<kT>::frag pf, floatx4 (&acc)[kD / 16 + 1]) {
+#pragma unroll
+  for (int dt = 0; dt < kD / 16; ++dt) acc[dt] = Slice<kT>::mfma(vf[dt], pf, acc[dt]);
+  acc[kD / 16] = Slice<kT>::mfma(splat<kT>(1.f), pf, acc[kD / 16]);
 }
 
 // Whether slice c of V is finite: the product with an all-zero P is NaN where V is not.
-template <int kD>
+template <int kD, int kT>
 __device__ __forceinline__ bool v_finite(uint32_t vs, int c) {
-  const half8 zero = as_half8(u32x4{0u, 0u, 0u, 0u});
   floatx4 chk = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int dt = 0; dt < kD / 16; ++dt) chk = mfma16x16x32(vt_frag<kD>(vs, c, dt), zero, chk);
+  for (int dt = 0; dt < kD / 16; ++dt)
+    chk = Slice<kT>::mfma(vt_frag<kD, kT>(vs, c, dt), splat<kT>(0.f), chk);
   // the file is compiled for NaN-free arithmetic: hide where the bits are from
   asm volatile("" : "+v"(chk));
   const u32x4 u = __builtin_bit_cast(u32x4, chk);
@@ -370,17 +427,19 @@ __device__ __forceinline__ bool v_finite(uint32_t vs, int c) {
 // in the matrix product would reach those rows.  The product runs on V with such values
 // replaced by zeros; then products of indicators (V is +inf or NaN / -inf or NaN; P is not zero)
 // count which of them each row sees, and put the infinities where they belong (both: NaN).
-template <int NB, int kD>
-__device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c, const half8 (&pf)[NB],
+template <int NB, int kD, int kT>
+__device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c,
+                                                 const typename Slice<kT>::frag (&pf)[NB],
                                                  floatx4 (&acc)[NB][kD / 16 + 1]) {
-  typedef unsigned short us8 __attribute__((ext_vector_type(8)));
-  constexpr int kT = kD / 16;
+  typedef typename Slice<kT>::bits bits;
+  typedef typename Slice<kT>::frag frag;
+  constexpr int kN = kD / 16;
 #pragma unroll
-  for (int dt = 0; dt < kT; ++dt) {
-    const us8 v = __builtin_bit_cast(us8, vt_frag<kD>(vs, c, dt));
-    us8 ok, inf[2];
+  for (int dt = 0; dt < kN; ++dt) {
+    const bits v = __builtin_bit_cast(bits, vt_frag<kD, kT>(vs, c, dt));
+    bits ok, inf[2];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < 4 * kT; ++e) {
       const unsigned short m = v[e] & 0x7fff;
       ok[e] = m < 0x7c00 ? v[e] : (unsigned short)0;
       inf[0][e] = m > 0x7c00 || v[e] == 0x7c00 ? (unsigned short)0x3c00 : (unsigned short)0;
@@ -388,14 +447,14 @@ __device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c, const half8
     }
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      acc[j][dt] = mfma16x16x32(__builtin_bit_cast(half8, ok), pf[j], acc[j][dt]);
-      us8 pi = __builtin_bit_cast(us8, pf[j]);
+      acc[j][dt] = Slice<kT>::mfma(__builtin_bit_cast(frag, ok), pf[j], acc[j][dt]);
+      bits pi = __builtin_bit_cast(bits, pf[j]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pi[e] = pi[e] ? (unsigned short)0x3c00 : (unsigned short)0;
+      for (int e = 0; e < 4 * kT; ++e) pi[e] = pi[e] ? (unsigned short)0x3c00 : (unsigned short)0;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const floatx4 n = mfma16x16x32(__builtin_bit_cast(half8, inf[i]), __builtin_bit_cast(half8, pi),
-                                       floatx4{0.f, 0.f, 0.f, 0.f});
+        const floatx4 n = Slice<kT>::mfma(__builtin_bit_cast(frag, inf[i]), __builtin_bit_cast(frag, pi),
+                                          floatx4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float x = n[r] > 0.f ? (i ? -__builtin_inff() : __builtin_inff()) : 0.f;
@@ -406,7 +465,7 @@ __device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c, const half8
     }
   }
 #pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j][kT] = mfma16x16x32(ones8(), pf[j], acc[j][kT]);
+  for (int j = 0; j < NB; ++j) acc[j][kN] = Slice<kT>::mfma(splat<kT>(1.f), pf[j], acc[j][kN]);
 }
 
 // x = cap_log2 * tanh(y), y = s * sm_scale / cap, in log2 units: tanh(y) = 1 - 2 / (1 + e^2y).
@@ -425,45 +484,52 @@ __device__ __forceinline__ float capped_series(const Params& p, float s) {
   return __builtin_fabsf(y) < 0.25f ? p.cap_log2 * t : capped(p, s);
 }
 
-// One resident tile (keys k0 .. k0 + 63) for this wave's rows.  s_pos, s_slope: of the wave's rows;
-// keys: bit k is set when key k0 + k is before the row's length and in the pool; kMasked: some
-// row may not see some key.
-template <int NB, int kD, int kMod, bool kMasked>
+// kSlices slices of 16 kT resident keys (k0 on) for this wave's rows.  s_pos, s_slope: of the wave's
+// rows; keys: bit k is set when key k0 + k is before the row's length and in the pool; kMasked:
+// some row may not see some key.
+template <int NB, int kD, int kMod, int kT, int kSlices, bool kMasked>
 __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t vs, int k0, uint64_t keys,
                                         int prefix, const int* s_pos, const float* s_slope, int col,
                                         int g, const half8 (&qf)[NB][kD / 32], float (&t_run)[NB],
                                         floatx4 (&acc)[NB][kD / 16 + 1]) {
+  typedef typename Slice<kT>::frag frag;
+  constexpr uint64_t kAll = ~0ull >> (64 - 16 * kT * kSlices);
+  constexpr int kE = 4 * kT;  // scores of a lane and row block
 #pragma unroll
-  for (int c = 0; c < kKTile / 32; ++c) {
+  for (int c = 0; c < kSlices; ++c) {
     // a uniform branch, never taken, between the slices: without it the compiler overlaps the
     // unrolled slices beyond the register file
     if (p.chunk < 0) break;
-    const int key0 = k0 + 32 * c + 4 * g;  // lane's key of (t, r): key0 + 16t + r
-    floatx4 s[NB][2];
-    auto bias = [&](int j, int t, int r) {
-      return -s_slope[16 * j + col] * __builtin_fabsf((float)(s_pos[16 * j + col] - key0 - 16 * t - r));
+    const int key0 = k0 + 16 * kT * c + 4 * g;  // lane's key of score e: key0 + 16 (e / 4) + e % 4
+    floatx4 s[NB][kT];
+    auto bias = [&](int j, int e) {
+      return -s_slope[16 * j + col] *
+             __builtin_fabsf((float)(s_pos[16 * j + col] - key0 - 16 * (e >> 2) - (e & 3)));
     };
 #pragma unroll
     for (int j = 0; j < NB; ++j)
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+      for (int e = 0; e < kE; ++e) s[j][e >> 2][e & 3] = kMod == kBias ? bias(j, e) : 0.f;
+    qk_slice<NB, kD, kT>(ks, c, qf, s);
+    frag vf[kD / 16];
+    if constexpr (NB == 1 && !kMasked) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[j][t][r] = kMod == kBias ? bias(j, t, r) : 0.f;
-    qk_slice<NB, kD>(ks, c, qf, s);
+      for (int dt = 0; dt < kD / 16; ++dt) vf[dt] = vt_frag<kD, kT>(vs, c, dt);
+    }
     if (kMod & kCap) {
       const bool series = p.cap_log2 > kExpCap * kLog2e;
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         if (series) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[j][e >> 2][e & 3] = capped_series(p, s[j][e >> 2][e & 3]);
+          for (int e = 0; e < kE; ++e) s[j][e >> 2][e & 3] = capped_series(p, s[j][e >> 2][e & 3]);
         } else {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[j][e >> 2][e & 3] = capped(p, s[j][e >> 2][e & 3]);
+          for (int e = 0; e < kE; ++e) s[j][e >> 2][e & 3] = capped(p, s[j][e >> 2][e & 3]);
         }
         if (kMod & kBias) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s[j][e >> 2][e & 3] += bias(j, e >> 2, e & 3);
+          for (int e = 0; e < kE; ++e) s[j][e >> 2][e & 3] += bias(j, e);
         }
       }
     }
@@ -472,24 +538,20 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
       for (int j = 0; j < NB; ++j) {
         const int pos = s_pos[16 * j + col];
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const int key = key0 + 16 * t + r;
-            const bool see = (key < prefix || (key <= pos && key > pos - p.window)) &&
-                             ((keys >> (key - k0)) & 1);
-            if (!see) s[j][t][r] = -__builtin_inff();
-          }
+        for (int e = 0; e < kE; ++e) {
+          const int key = key0 + 16 * (e >> 2) + (e & 3);
+          const bool see = (key < prefix || (key <= pos && key > pos - p.window)) &&
+                           ((keys >> (key - k0)) & 1);
+          if (!see) s[j][e >> 2][e & 3] = -__builtin_inff();
+        }
       }
-    } else if (keys != ~0ull) {  // missing table entries
-      const uint32_t bits = (uint32_t)(keys >> (32 * c)) >> (4 * g);
+    } else if (keys != kAll) {  // missing table entries
+      const uint32_t here = (uint32_t)(keys >> (16 * kT * c)) >> (4 * g);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (!((bits >> (16 * t + r)) & 1)) s[j][t][r] = -__builtin_inff();
+        for (int e = 0; e < kE; ++e)
+          if (!((here >> (16 * (e >> 2) + (e & 3))) & 1)) s[j][e >> 2][e & 3] = -__builtin_inff();
     }
     // Online softmax with a lazily moved reference max, kept as the threshold t = max + slack in
     // score units: it moves only when a score exceeds it (p <= 2^8, exact in fp16; sums in fp32).
@@ -497,8 +559,9 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
     float lmax[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
-      const float x = fmaxf(fmaxf(s[j][0][0], s[j][0][1]), fmaxf(s[j][0][2], s[j][0][3]));
-      lmax[j] = fmaxf(fmaxf(fmaxf(s[j][1][0], s[j][1][1]), fmaxf(s[j][1][2], s[j][1][3])), x);
+      lmax[j] = fmaxf(fmaxf(s[j][0][0], s[j][0][1]), fmaxf(s[j][0][2], s[j][0][3]));
+      if constexpr (kT == 2)
+        lmax[j] = fmaxf(fmaxf(fmaxf(s[j][1][0], s[j][1][1]), fmaxf(s[j][1][2], s[j][1][3])), lmax[j]);
       move |= lmax[j] > t_run[j];
     }
     if (__builtin_amdgcn_ballot_w64(move)) {
@@ -514,69 +577,114 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
       }
     }
     // P is rounded to fp16 for the matrix cores; the sums take the rounded values too.
-    half8 pf[NB];
+    frag pf[NB];
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const float mc = __builtin_fmaf(t_run[j], p.scale_log2, -p.lazy_log2);
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          pf[j][4 * t + r] = (half_t)fast_exp2(__builtin_fmaf(s[j][t][r], p.scale_log2, -mc));
+      for (int e = 0; e < kE; ++e)
+        pf[j][e] = (half_t)fast_exp2(__builtin_fmaf(s[j][e >> 2][e & 3], p.scale_log2, -mc));
     }
-    if (kMasked && !v_finite<kD>(vs, c))
-      pv_slice_careful<NB, kD>(vs, c, pf, acc);
-    else
-      pv_slice<NB, kD>(vs, c, pf, acc);
+    if constexpr (NB == 1 && !kMasked) {
+      pv_read<kD, kT>(vf, pf[0], acc[0]);
+    } else {
+      if (kMasked && !v_finite<kD, kT>(vs, c))
+        pv_slice_careful<NB, kD, kT>(vs, c, pf, acc);
+      else
+        pv_slice<NB, kD, kT>(vs, c, pf, acc);
+    }
   }
 }
 
+// Q^T fragments of the wave's row blocks, rows r0 on (MFMA i takes d = 32 i + 8 g + s in reduction
+// slot 8 g + s), and their positions and biases into LDS.
 template <int NB, int kD, int kMod>
-__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
-  typedef Tile<kD> T;
-  constexpr int kRowsPerWave = 16 * NB;
-  constexpr int kRows = kWaves * kRowsPerWave;
-  __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
-  __shared__ int s_pos[kRows];      // position of each query row, -1 for rows without a token
-  __shared__ float s_slope[kRows];  // its distance bias in score units
+__device__ __forceinline__ void load_rows(const Params& p, const Row& row, int b, int kvh, int r0, int col,
+                                          int g, half8 (&qf)[NB][kD / 32], int* s_pos, float* s_slope) {
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    const int r = r0 + 16 * j + col;
+    const int t = div_by(r, p.group_div);
+    const int h = kvh * p.group + r - t * p.group;
+    const int pos = row.start + t;
+    const bool ok = t < p.chunk && pos >= 0 && pos < row.len;
+    const half_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)(ok ? t : 0) * p.q_st + (int64_t)h * p.q_sh;
+#pragma unroll
+    for (int i = 0; i < kD / 32; ++i) {
+      u32x4 v = {0u, 0u, 0u, 0u};
+      if (ok && !p.q_zero && 32 * i + 8 * g < p.head_dim) v = *(const u32x4*)(src + 32 * i + 8 * g);
+      qf[j][i] = as_half8(v ^ p.q_sign);
+    }
+    if (g == 0) {
+      s_pos[16 * j + col] = ok ? pos : -1;
+      if (kMod & kBias) s_slope[16 * j + col] = p.slopes[h] * p.slope_mul;
+    }
+  }
+}
 
-  const int tid = threadIdx.x;
-  const int lane = tid & 63;
-  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 15;
-  const int g = lane >> 4;
-  const int kvh = blockIdx.x % p.num_kv_heads;
+// The part of the work of a workgroup: its batch row, row tile and key tiles first .. first + n - 1 of
+// the span's order.  False where there is nothing to do.
+struct Job {
+  int b, kvh, r0, parts, first, n;
+  Row row;
+  Span span;
+};
+__device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows, Job& job) {
+  job.kvh = blockIdx.x % p.num_kv_heads;
   const int item = blockIdx.x / p.num_kv_heads;
-  int b, tile, part = 0, parts = 1;
+  int tile, part = 0;
+  job.parts = 1;
   if (p.part_o) {
-    const Share s = find_share(p, item, lane);
-    if (s.b < 0) return;  // past the list
-    b = s.b;
-    const RowTiles rt = row_tiles_of(p, row_of(p, b));
+    const Share s = find_share(p, item, tid & 63);
+    if (s.b < 0) return false;  // past the list
+    job.b = s.b;
+    const RowTiles rt = row_tiles_of(p, row_of(p, job.b));
     int at = item - s.before;
-    if (at == 0 && kvh == 0 && tid < 2) p.shares[2 * b + tid] = tid ? s.parts : s.before;
+    if (at == 0 && job.kvh == 0 && tid < 2) p.shares[2 * job.b + tid] = tid ? s.parts : s.before;
     if (at < rt.count * s.parts) {
       part = at / rt.count;
-      parts = s.parts;
+      job.parts = s.parts;
       tile = rt.first + rt.count - 1 - (at - part * rt.count);
     } else {  // a row tile without tokens
       at -= rt.count * s.parts;
       tile = at < rt.first ? at : at + rt.count;
     }
   } else {  // the last row tiles see the most keys: first
-    b = item % p.batch;
+    job.b = item % p.batch;
     tile = p.row_tiles - 1 - item / p.batch;
   }
-  const int r0 = tile * kRows;
-
-  const Row row = row_of(p, b);
+  job.r0 = tile * tile_rows;
+  job.row = row_of(p, job.b);
   int lo, hi;
-  row_positions(p, row, r0, r0 + kRows - 1, lo, hi);
-  const Span span = span_of(p, row, lo, hi);
-  const int size = (span.n + parts - 1) / parts;
-  const int first = min(part * size, span.n);
-  const int n = min(size, span.n - first);
-  if (parts > 1 && n == 0) return;  // a short list in few pieces: the other kernel reads no more
+  row_positions(p, job.row, job.r0, job.r0 + tile_rows - 1, lo, hi);
+  job.span = span_of(p, job.row, lo, hi);
+  const int size = (job.span.n + job.parts - 1) / job.parts;
+  job.first = min(part * size, job.span.n);
+  job.n = min(size, job.span.n - job.first);
+  // a short list in few pieces: the other kernel reads no more
+  return job.parts == 1 || job.n > 0;
+}
+
+// Many rows: the waves share the tiles, each with rows of its own.
+template <int NB, int kD, int kMod>
+__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
+  typedef Tile<kD> T;
+  constexpr int kRowsPerWave = 16 * NB;
+  constexpr int kRows = kWaves * kRowsPerWave;
+  __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
+  __shared__ int s_pos[kRows];  // position of each query row, -1 for rows without a token
+  __shared__ float s_slope[kMod & kBias ? kRows : 1];  // its distance bias in score units
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15;
+  const int g = lane >> 4;
+  Job job;
+  if (!find_job(p, tid, kRows, job)) return;
+  const int b = job.b, kvh = job.kvh, r0 = job.r0, first = job.first, n = job.n;
+  const Row& row = job.row;
+  const Span& span = job.span;
 
   // The table entry of key `lane` of key tile i, -1 where it is not to be read.
   auto entry_of = [&](int i) -> int {
@@ -594,36 +702,17 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
 
   int row_next = pool_row(0, entry_of(0));
-  issue_tile<kD>(p, kbase, vbase, stages, row_next, w, lane);
+  issue_tile<kD>(p, kbase, vbase, stages, row_next, 16 * w, w, lane);
   uint64_t keys = __builtin_amdgcn_ballot_w64(row_next >= 0), keys_next = 0;
   row_next = pool_row(1, entry_of(1));
   keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
-  issue_tile<kD>(p, kbase, vbase, stages + T::kStage, row_next, w, lane);
+  issue_tile<kD>(p, kbase, vbase, stages + T::kStage, row_next, 16 * w, w, lane);
   int entry = entry_of(2);
 
-  // Q^T fragments: MFMA i takes d = 32 i + 8 g + s in reduction slot 8 g + s.
   half8 qf[NB][kD / 32];
-#pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int r = r0 + kRowsPerWave * w + 16 * j + col;
-    const int t = div_by(r, p.group_div);
-    const int h = kvh * p.group + r - t * p.group;
-    const int pos = row.start + t;
-    const bool ok = t < p.chunk && pos >= 0 && pos < row.len;
-    const half_t* src = p.q + (int64_t)b * p.q_sb + (int64_t)(ok ? t : 0) * p.q_st + (int64_t)h * p.q_sh;
-#pragma unroll
-    for (int i = 0; i < kD / 32; ++i) {
-      u32x4 v = {0u, 0u, 0u, 0u};
-      if (ok && !p.q_zero && 32 * i + 8 * g < p.head_dim) v = *(const u32x4*)(src + 32 * i + 8 * g);
-      qf[j][i] = as_half8(v ^ p.q_sign);
-    }
-    if (g == 0) {
-      s_pos[kRowsPerWave * w + 16 * j + col] = ok ? pos : -1;
-      if (kMod & kBias) s_slope[kRowsPerWave * w + 16 * j + col] = p.slopes[h] * p.slope_mul;
-    }
-  }
-  const int* w_pos = s_pos + kRowsPerWave * w;
-  const float* w_slope = s_slope + kRowsPerWave * w;
+  int* w_pos = s_pos + kRowsPerWave * w;
+  float* w_slope = s_slope + (kMod & kBias ? kRowsPerWave * w : 0);
+  load_rows<NB, kD, kMod>(p, row, b, kvh, r0 + kRowsPerWave * w, col, g, qf, w_pos, w_slope);
   int wlo, whi;  // positions of this wave's tokens
   row_positions(p, row, r0 + kRowsPerWave * w, r0 + kRowsPerWave * (w + 1) - 1, wlo, whi);
 
@@ -644,7 +733,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     row_next = pool_row(i + 1, entry);
     keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
     entry = entry_of(i + 2);
-    issue_tile<kD>(p, kbase, vbase, stages + ((i + 1) & 1) * T::kStage, row_next, w, lane);
+    issue_tile<kD>(p, kbase, vbase, stages + ((i + 1) & 1) * T::kStage, row_next, 16 * w, w, lane);
   };
   const uint32_t ks = lds_addr(stages) + k_lane<kD>(col, g);
   const uint32_t vs = lds_addr(stages) + T::kBytes + v_lane<kD>(col, g);
@@ -653,22 +742,22 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     copy_next(i);
     const int k0 = span.tile(first + i) * kKTile;
     if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
-      consume<NB, kD, kMod, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
-                                  row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
+      consume<NB, kD, kMod, 2, 2, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
+                                        row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
     keys = keys_next;
     stage_barrier();
   }
   for (; i < n; ++i) {
     copy_next(i);
     if (wlo <= whi)
-      consume<NB, kD, kMod, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
-                                   span.tile(first + i) * kKTile, keys, row.prefix, w_pos, w_slope, col, g,
-                                   qf, t_run, acc);
+      consume<NB, kD, kMod, 2, 2, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
+                                         span.tile(first + i) * kKTile, keys, row.prefix, w_pos, w_slope,
+                                         col, g, qf, t_run, acc);
     keys = keys_next;
     stage_barrier();
   }
 
-  if (parts > 1) {
+  if (job.parts > 1) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       const int rl = kRowsPerWave * w + 16 * j + col;
@@ -709,6 +798,165 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     const u32x4 v = *(const u32x4*)(ostage + rl * kORow + 16 * oc);
     if (t < p.chunk && oc < p.d_chunks)
       *(u32x4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * oc) = v;
+  }
+}
+
+// Few rows (at most 16 NB): every wave has all of them and takes 16 keys of each tile, those that it
+// copies itself, so the waves run without barriers, each waiting for its own copies only, and
+// are added up through LDS at the end.  Bound by the stream of K and V: with the rows of one
+// wave and shared tiles, 2.9 TB/s.  The table entries come through LDS as well (an ordinary load
+// in the loop would make the compiler wait for every copy): their copies run two tiles ahead of
+// the keys' copies, which run one tile ahead of the sums.
+template <int NB, int kD, int kMod>
+__global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_kernel(Params p) {
+  typedef Tile<kD> T;
+  constexpr int kRows = 16 * NB;
+  constexpr int kEnts = 4;
+  __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
+  __shared__ int s_ent[kWaves][kEnts][64];
+  __shared__ int s_pos[kWaves][kRows];
+  __shared__ float s_slope[kWaves][kMod & kBias ? kRows : 1];
+  __shared__ float s_ml[kWaves][kRows][2];
+
+  const int tid = threadIdx.x;
+  const int lane = tid & 63;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15;
+  const int g = lane >> 4;
+  Job job;
+  if (!find_job(p, tid, kRows, job)) return;
+  const int b = job.b, kvh = job.kvh, r0 = job.r0, first = job.first, n = job.n;
+  const Row& row = job.row;
+  const Span& span = job.span;
+
+  // Lane l stands for key 16w + l % 16 of a tile.
+  auto key_of = [&](int i) { return span.tile(first + i) * kKTile + 16 * w + col; };
+  auto copy_entries = [&](int i) {
+    const int key = key_of(i);
+    const int blk = div_by(key, p.block_div);
+    const int32_t* src = i < n && key < row.len && blk < p.max_blocks_per_seq
+                             ? p.block_table + (int64_t)b * p.bt_stride + blk : &g_no_block;
+    lds_copy4_global(src, lds_addr(&s_ent[w][i & (kEnts - 1)][0]));
+  };
+  const char* kbase = (const char*)(p.k_cache + (int64_t)kvh * p.head_dim);
+  const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
+  auto copy_tile = [&](int i) -> uint32_t {  // its keys in the pool, one bit each
+    const int key = key_of(i);
+    const int slot = key - div_by(key, p.block_div) * p.block_size;
+    const int entry = s_ent[w][i & (kEnts - 1)][lane];
+    const int at = entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
+    issue_tile<kD>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0) & 0xffffu;
+  };
+
+#pragma unroll
+  for (int i = 0; i < 3; ++i) copy_entries(i);
+  half8 qf[NB][kD / 32];
+  load_rows<NB, kD, kMod>(p, row, b, kvh, r0, col, g, qf, s_pos[w], s_slope[w]);
+  // also for the compiler, which would otherwise wait for every copy at the first use of Q
+  wait_vmcnt<0>();
+  asm volatile("" ::: "memory");
+  uint32_t keys = 0, keys_next = 0;
+  if (n > 0) keys = copy_tile(0);
+  if (n > 1) {
+    copy_entries(3);
+    keys_next = copy_tile(1);
+  }
+
+  float t_run[NB];
+  floatx4 acc[NB][kD / 16 + 1];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    t_run[j] = kNegBig;
+#pragma unroll
+    for (int dt = 0; dt <= kD / 16; ++dt) acc[j][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
+  }
+  const uint32_t ks = lds_addr(stages) + 16 * w * T::kRow + k_lane<kD>(col, g);
+  const uint32_t vs = lds_addr(stages) + T::kBytes + 16 * w * T::kRow + v_lane<kD>(col, g);
+  // behind tile i: the entries of tile i + 3 and tile i + 1 are on their way
+  auto arrive = [&](int i) {
+    if (i + 1 < n)
+      wait_copies<2 * T::kCopies + 1>();
+    else
+      wait_copies<0>();
+  };
+  auto advance = [&](int i) {
+    keys = keys_next;
+    if (i + 2 < n) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of this stage are done
+      copy_entries(i + 4);
+      keys_next = copy_tile(i + 2);
+    }
+  };
+  int i = 0;
+  for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
+    arrive(i);
+    consume<NB, kD, kMod, 1, 1, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
+                                      span.tile(first + i) * kKTile + 16 * w, keys, row.prefix, s_pos[w],
+                                      s_slope[w], col, g, qf, t_run, acc);
+    advance(i);
+  }
+  for (; i < n; ++i) {
+    arrive(i);
+    consume<NB, kD, kMod, 1, 1, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
+                                       span.tile(first + i) * kKTile + 16 * w, keys, row.prefix, s_pos[w],
+                                       s_slope[w], col, g, qf, t_run, acc);
+    advance(i);
+  }
+
+  // Add the waves up, one row block at a time: O and the sums relative to the waves' own maxima.
+  float* cmb = (float*)stages;  // [wave][16][kD]
+  static_assert(kWaves * 16 * kD * 4 <= 2 * T::kStage, "a row block of every wave fits the stages");
+  if (g == 0) {
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+      s_ml[w][16 * j + col][0] = __builtin_fmaf(t_run[j], p.scale_log2, -p.lazy_log2);
+      s_ml[w][16 * j + col][1] = acc[j][kD / 16][0];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    if (r0 + 16 * j >= p.chunk * p.group) break;
+    __syncthreads();
+#pragma unroll
+    for (int dt = 0; dt < kD / 16; ++dt)
+      *(floatx4*)(cmb + (w * 16 + col) * kD + 16 * dt + 4 * g) = acc[j][dt];
+    __syncthreads();
+    for (int x = tid; x < 16 * kD / 4; x += kThreads) {
+      const int c = x / (kD / 4), d = x % (kD / 4) * 4;
+      const int rl = 16 * j + c, r = r0 + rl;
+      const int t = div_by(r, p.group_div);
+      if (t >= p.chunk) continue;
+      float m = kNegBig;
+#pragma unroll
+      for (int ww = 0; ww < kWaves; ++ww)
+        if (__builtin_bit_cast(uint32_t, s_ml[ww][rl][1]) != 0) m = fmaxf(m, s_ml[ww][rl][0]);
+      float l = 0.f;
+      floatx4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ww = 0; ww < kWaves; ++ww) {
+        const float lw = s_ml[ww][rl][1];
+        if (__builtin_bit_cast(uint32_t, lw) == 0) continue;  // saw no key (a NaN is not 0)
+        const float e = fast_exp2(s_ml[ww][rl][0] - m);
+        l += lw * e;
+        o += *(const floatx4*)(cmb + (ww * 16 + c) * kD + d) * e;
+      }
+      const bool there = s_pos[0][rl] >= 0;
+      if (job.parts > 1) {
+        if (!there) continue;
+        const int64_t slot = (int64_t)blockIdx.x * p.part_rows + rl;
+        *(floatx4*)(p.part_o + slot * kD + d) = o;
+        if (d == 0) {
+          p.part_ml[slot * 2] = m;
+          p.part_ml[slot * 2 + 1] = l;
+        }
+      } else if (d < p.head_dim) {
+        const float inv = there && __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
+        const int h = kvh * p.group + r - t * p.group;
+        *(half4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + d) =
+            to_half4(o * inv);
+      }
+    }
   }
 }
 
@@ -779,8 +1027,10 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
 // results' rows of the parts (0: not cut).
 constexpr int64_t kMaxWgs = (1 << 24) - 1;  // a launch takes fewer than 2^32 threads along x
 struct Plan {
+  bool narrow;
   int nb;
   int64_t row_tiles, wgs, target, part_rows, width;
+  int64_t tile_rows() const { return narrow ? 16 * nb : 64 * nb; }
   size_t bytes(int64_t batch) const {
     return (size_t)((target + wgs) * part_rows * (width + 2) + 2 * batch) * sizeof(float);
   }
@@ -790,11 +1040,16 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
   const int64_t rows = chunk * (num_q_heads / num_kv_heads);
   Plan pl;
   pl.width = head_dim <= 64 ? 64 : 128;
-  pl.nb = (int)std::min<int64_t>((rows + 63) / 64, kMaxNb);
-  pl.row_tiles = (rows + 64 * pl.nb - 1) / (64 * pl.nb);
+  pl.narrow = rows <= 64;
+  const int64_t blocks = (rows + 15) / 16;
+  pl.nb = pl.narrow ? (blocks <= 2 ? (int)blocks : 4) : rows <= 128 ? 2 : 3;
+  const int64_t tile_rows = pl.tile_rows();
+  pl.row_tiles = (rows + tile_rows - 1) / tile_rows;
   pl.wgs = batch * num_kv_heads * pl.row_tiles;
-  pl.target = pl.wgs < kSlots && num_tokens > kMinPart * kKTile ? kSlots : 0;
-  pl.part_rows = pl.target ? std::min<int64_t>(rows, 64 * pl.nb) : 0;
+  // workgroups resident at once: two per CU, four of the narrow 64-wide form
+  const int64_t slots = pl.narrow && pl.width == 64 && pl.nb < 4 ? 1024 : 512;
+  pl.target = pl.wgs < slots && num_tokens > kMinPart * kKTile ? slots : 0;
+  pl.part_rows = pl.target ? std::min<int64_t>(rows, tile_rows) : 0;
   return pl;
 }
 
@@ -804,22 +1059,26 @@ static bool sizes_ok(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t 
 }
 
 template <int kD, int kMod>
-static void launch(int nb, dim3 grid, hipStream_t st, const Params& p) {
+static void launch(const Plan& pl, dim3 grid, hipStream_t st, const Params& p) {
   const dim3 block(kThreads);
-  if (nb == 1)
-    hipLaunchKernelGGL((chunk_kernel<1, kD, kMod>), grid, block, 0, st, p);
-  else if (nb == 2)
+  if (pl.narrow && pl.nb == 1)
+    hipLaunchKernelGGL((narrow_kernel<1, kD, kMod>), grid, block, 0, st, p);
+  else if (pl.narrow && pl.nb == 2)
+    hipLaunchKernelGGL((narrow_kernel<2, kD, kMod>), grid, block, 0, st, p);
+  else if (pl.narrow)
+    hipLaunchKernelGGL((narrow_kernel<4, kD, kMod>), grid, block, 0, st, p);
+  else if (pl.nb == 2)
     hipLaunchKernelGGL((chunk_kernel<2, kD, kMod>), grid, block, 0, st, p);
   else
     hipLaunchKernelGGL((chunk_kernel<3, kD, kMod>), grid, block, 0, st, p);
 }
 template <int kD>
-static void launch(int mod, int nb, dim3 grid, hipStream_t st, const Params& p) {
+static void launch(int mod, const Plan& pl, dim3 grid, hipStream_t st, const Params& p) {
   switch (mod) {
-    case 0: launch<kD, 0>(nb, grid, st, p); break;
-    case kCap: launch<kD, kCap>(nb, grid, st, p); break;
-    case kBias: launch<kD, kBias>(nb, grid, st, p); break;
-    default: launch<kD, kCap | kBias>(nb, grid, st, p); break;
+    case 0: launch<kD, 0>(pl, grid, st, p); break;
+    case kCap: launch<kD, kCap>(pl, grid, st, p); break;
+    case kBias: launch<kD, kBias>(pl, grid, st, p); break;
+    default: launch<kD, kCap | kBias>(pl, grid, st, p); break;
   }
 }
 
@@ -945,7 +1204,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
     return FI_ERR_UNSUPPORTED;
   }
   if (pl.target && (!workspace || workspace_bytes < pl.bytes(batch))) pl.target = 0;
-  p.tile_rows = 64 * pl.nb;
+  p.tile_rows = (int)pl.tile_rows();
   p.tile_div = fast_div((uint32_t)p.tile_rows);
   p.row_tiles = (int)pl.row_tiles;
   if (pl.target) {
@@ -965,9 +1224,9 @@ extern "C" int fi_paged_chunk_attention_fwd(
   const hipStream_t st = (hipStream_t)stream;
   const int mod = (softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0);
   if (pl.width == 64)
-    launch<64>(mod, pl.nb, grid, st, p);
+    launch<64>(mod, pl, grid, st, p);
   else
-    launch<128>(mod, pl.nb, grid, st, p);
+    launch<128>(mod, pl, grid, st, p);
   const int rc = check_launch(fn);
   if (rc != FI_OK || !pl.target) return rc;
   const int64_t merge_rows = kMergeThreads / (pl.width / 4);

@@ -99,7 +99,7 @@ def test_chunk_workspace_size(lib):
         group, hkv = rng.randint(1, 16), rng.randint(1, 16)
         sizes = [size(batch, new, group * hkv, hkv, n, 128) for n in (64, 300, 1000, 5000, 1 << 17, 1 << 22)]
         assert sizes == sorted(sizes)
-        assert sizes[-1] <= 1024 * min(192, new * group) * 130 * 4 + 8 * batch
+        assert sizes[-1] <= 2048 * min(192, new * group) * 130 * 4 + 8 * batch
 
 
 @pytest.mark.parametrize("bad,rc,text", [
@@ -182,7 +182,7 @@ def test_m0_is_only_set_by_the_copy_helper(tmp_path):
     for i, ln in enumerate(lines):
         if re.search(r"\bm0\b", ln):
             assert re.fullmatch(r"s_mov_b32 m0, s\d+", ln), ln
-            assert lines[i + 1] == "s_nop 0" and lines[i + 2].startswith("global_load_lds_dwordx4"), ln
+            assert lines[i + 1] == "s_nop 0" and lines[i + 2].startswith("global_load_lds_dword"), ln
             copies += 1
     assert copies == sum(ln.startswith("global_load_lds") for ln in lines) > 0
 
