@@ -175,11 +175,12 @@ __device__ __forceinline__ RowTiles row_tiles_of(const Params& p, const Row& row
   return r;
 }
 
-// Every workgroup finds its part by itself, from the lengths on the device: the part size is all
-// key tiles to visit over the parts aimed at (kMinPart at least), each row tile of batch row b is
-// cut into parts(b) = ceil(its longest list / size) equal pieces, and the work list is, for each
-// b, its parts (row tile fastest, so that neighbours read the same keys), then its row tiles
-// without tokens, one each.  The batch row of list place `item` (-1 past the list), the
+// Every workgroup finds its part by itself, from the lengths on the device: each row tile of batch
+// row b is cut into parts(b) = ceil(its longest list / size) equal pieces, with the size at which
+// about `target` parts, what the device holds at once, take all key tiles (a few steps from below;
+// one more round of workgroups, however few, takes as long as the first); the work list is, for
+// each b, its parts (row tile fastest, so that neighbours read the same keys), then its row
+// tiles without tokens, one each.  The batch row of list place `item` (-1 past the list), the
 // places before it and its parts.  Wave-wide; lanes hold batch rows.
 struct Share {
   int b, before, parts;
@@ -187,18 +188,29 @@ struct Share {
 __device__ __forceinline__ int wave_sum(int v) {
 #pragma unroll
   for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-  return v;
+  return __builtin_amdgcn_readfirstlane(v);
 }
 __device__ __forceinline__ Share find_share(const Params& p, int item, int lane) {
   auto tiles_of = [&](int i) { return i < p.batch ? row_tiles_of(p, row_of(p, i)) : RowTiles{0, 0, 0}; };
   const RowTiles t0 = tiles_of(lane);
   int total = t0.count * t0.n;
-  for (int i = lane + 64; i < p.batch; i += 64) {
-    const RowTiles t = tiles_of(i);
+  for (int i0 = 64; i0 < p.batch; i0 += 64) {
+    const RowTiles t = tiles_of(i0 + lane);
     total += t.count * t.n;
   }
   total = wave_sum(total) * p.num_kv_heads;
-  const int size = max((total + p.target - 1) / p.target, kMinPart);
+  int size = max((total + p.target - 1) / p.target, kMinPart);
+  for (int step = 0; step < 4; ++step) {
+    int wgs = t0.count * ((t0.n + size - 1) / size);
+    for (int i0 = 64; i0 < p.batch; i0 += 64) {
+      const RowTiles t = tiles_of(i0 + lane);
+      wgs += t.count * ((t.n + size - 1) / size);
+    }
+    wgs = wave_sum(wgs) * p.num_kv_heads;
+    if (wgs <= p.target) break;
+    size = max((size * wgs + p.target - 1) / p.target, size + 1);
+  }
+  size = __builtin_amdgcn_readfirstlane(size);
   Share s = {-1, 0, 1};
   int before = 0;
   for (int i0 = 0; i0 < p.batch; i0 += 64) {
