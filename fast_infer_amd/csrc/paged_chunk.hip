@@ -475,6 +475,7 @@ __device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c,
         }
       }
     }
+    __builtin_amdgcn_sched_barrier(0);  // one step's registers at a time
   }
 #pragma unroll
   for (int j = 0; j < NB; ++j) acc[j][kN] = Slice<kT>::mfma(splat<kT>(1.f), pf[j], acc[j][kN]);
@@ -686,6 +687,8 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
   __shared__ int s_pos[kRows];  // position of each query row, -1 for rows without a token
   __shared__ float s_slope[kMod & kBias ? kRows : 1];  // its distance bias in score units
+  __shared__ int s_ent[4][kWaves][64];
+  __shared__ __attribute__((aligned(8))) uint16_t s_keys[2][kWaves];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -698,29 +701,31 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const Row& row = job.row;
   const Span& span = job.span;
 
-  // The table entry of key `lane` of key tile i, -1 where it is not to be read.
-  auto entry_of = [&](int i) -> int {
-    const int key = span.tile(first + i) * kKTile + lane;
+  // Lane l of wave w holds the table entry, then the pool row, of key 16w + l % 16 of a tile; the
+  // entries come through LDS: an ordinary load in the loop would make the compiler wait for every
+  // copy.  Their copies run two tiles ahead of the keys'.
+  auto key_of = [&](int i) { return span.tile(first + i) * kKTile + 16 * w + col; };
+  auto copy_entries = [&](int i) {
+    const int key = key_of(i);
     const int blk = div_by(key, p.block_div);
-    return i < n && key < row.len && blk < p.max_blocks_per_seq
-               ? p.block_table[(int64_t)b * p.bt_stride + blk] : -1;
-  };
-  auto pool_row = [&](int i, int entry) -> int {
-    const int key = span.tile(first + i) * kKTile + lane;
-    const int slot = key - div_by(key, p.block_div) * p.block_size;
-    return entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
+    const int32_t* src = i < n && key < row.len && blk < p.max_blocks_per_seq
+                             ? p.block_table + (int64_t)b * p.bt_stride + blk : &g_no_block;
+    lds_copy4_global(src, lds_addr(&s_ent[i & 3][w][0]));
   };
   const char* kbase = (const char*)(p.k_cache + (int64_t)kvh * p.head_dim);
   const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
+  auto copy_tile = [&](int i) {  // with its keys in the pool, 16 bits a wave
+    const int key = key_of(i);
+    const int slot = key - div_by(key, p.block_div) * p.block_size;
+    const int entry = s_ent[i & 3][w][lane];
+    const int at = entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
+    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
+    if (lane == 0) s_keys[i & 1][w] = (uint16_t)there;
+    issue_tile<kD>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
+  };
 
-  int row_next = pool_row(0, entry_of(0));
-  issue_tile<kD>(p, kbase, vbase, stages, row_next, 16 * w, w, lane);
-  uint64_t keys = __builtin_amdgcn_ballot_w64(row_next >= 0), keys_next = 0;
-  row_next = pool_row(1, entry_of(1));
-  keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
-  issue_tile<kD>(p, kbase, vbase, stages + T::kStage, row_next, 16 * w, w, lane);
-  int entry = entry_of(2);
-
+#pragma unroll
+  for (int i = 0; i < 3; ++i) copy_entries(i);
   half8 qf[NB][kD / 32];
   int* w_pos = s_pos + kRowsPerWave * w;
   float* w_slope = s_slope + (kMod & kBias ? kRowsPerWave * w : 0);
@@ -736,36 +741,40 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
 #pragma unroll
     for (int dt = 0; dt <= kD / 16; ++dt) acc[j][dt] = floatx4{0.f, 0.f, 0.f, 0.f};
   }
+  wait_copies<0>();
+  copy_tile(0);
+  copy_entries(3);
+  copy_tile(1);
   stage_barrier();
 
   // Tile i lies in stage i % 2.  While it is consumed, tile i + 1 is copied into the other stage
-  // (whose readers have passed the last barrier) and the table entries of tile i + 2 are read.
-  auto copy_next = [&](int i) {
-    if (i == 0) return;  // the first two are on their way
-    row_next = pool_row(i + 1, entry);
-    keys_next = __builtin_amdgcn_ballot_w64(row_next >= 0);
-    entry = entry_of(i + 2);
-    issue_tile<kD>(p, kbase, vbase, stages + ((i + 1) & 1) * T::kStage, row_next, 16 * w, w, lane);
+  // (whose readers have passed the last barrier).
+  auto copy_next = [&](int i) -> uint64_t {  // the keys of tile i
+    const uint64_t k = *(const uint64_t*)s_keys[i & 1];
+    if (i > 0) {  // the first two are on their way
+      copy_entries(i + 3);
+      copy_tile(i + 1);
+    }
+    return ((uint64_t)__builtin_amdgcn_readfirstlane((int)(k >> 32)) << 32) |
+           (uint32_t)__builtin_amdgcn_readfirstlane((int)k);
   };
   const uint32_t ks = lds_addr(stages) + k_lane<kD>(col, g);
   const uint32_t vs = lds_addr(stages) + T::kBytes + v_lane<kD>(col, g);
   int i = 0;
   for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
-    copy_next(i);
+    const uint64_t keys = copy_next(i);
     const int k0 = span.tile(first + i) * kKTile;
     if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
       consume<NB, kD, kMod, 2, 2, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
                                         row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
-    keys = keys_next;
     stage_barrier();
   }
   for (; i < n; ++i) {
-    copy_next(i);
+    const uint64_t keys = copy_next(i);
     if (wlo <= whi)
       consume<NB, kD, kMod, 2, 2, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
                                          span.tile(first + i) * kKTile, keys, row.prefix, w_pos, w_slope,
                                          col, g, qf, t_run, acc);
-    keys = keys_next;
     stage_barrier();
   }
 
