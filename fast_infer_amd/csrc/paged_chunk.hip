@@ -609,6 +609,21 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
   }
 }
 
+// A tile that needs masks, one row block at a time: with all blocks at once the accumulators spill,
+// and the waits for the reloads wait for the next tile's copies too.
+template <int NB, int kD, int kMod, int kT, int kSlices>
+__device__ __forceinline__ void consume_masked(const Params& p, uint32_t ks, uint32_t vs, int k0, uint64_t keys,
+                                               int prefix, const int* s_pos, const float* s_slope, int col,
+                                               int g, const half8 (&qf)[NB][kD / 32], float (&t_run)[NB],
+                                               floatx4 (&acc)[NB][kD / 16 + 1]) {
+#pragma unroll
+  for (int j = 0; j < NB; ++j)
+    consume<1, kD, kMod, kT, kSlices, true>(
+        p, ks, vs, k0, keys, prefix, s_pos + 16 * j, s_slope + (kMod & kBias ? 16 * j : 0), col, g,
+        reinterpret_cast<const half8(&)[1][kD / 32]>(qf[j]), reinterpret_cast<float(&)[1]>(t_run[j]),
+        reinterpret_cast<floatx4(&)[1][kD / 16 + 1]>(acc[j]));
+}
+
 // Q^T fragments of the wave's row blocks, rows r0 on (MFMA i takes d = 32 i + 8 g + s in reduction
 // slot 8 g + s), and their positions and biases into LDS.
 template <int NB, int kD, int kMod>
@@ -765,7 +780,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     const uint64_t keys = copy_next(i);
     const int k0 = span.tile(first + i) * kKTile;
     if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
-      consume<NB, kD, kMod, 2, 2, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
+      consume_masked<NB, kD, kMod, 2, 2>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
                                         row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
     stage_barrier();
   }
@@ -912,7 +927,7 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
   int i = 0;
   for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
     arrive(i);
-    consume<NB, kD, kMod, 1, 1, true>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
+    consume_masked<NB, kD, kMod, 1, 1>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
                                       span.tile(first + i) * kKTile + 16 * w, keys, row.prefix, s_pos[w],
                                       s_slope[w], col, g, qf, t_run, acc);
     advance(i);
