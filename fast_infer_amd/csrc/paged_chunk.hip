@@ -185,10 +185,21 @@ __device__ __forceinline__ RowTiles row_tiles_of(const Params& p, const Row& row
 struct Share {
   int b, before, parts;
 };
-__device__ __forceinline__ int wave_sum(int v) {
-#pragma unroll
-  for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-  return __builtin_amdgcn_readfirstlane(v);
+// Inclusive sums over the lanes (row shifts, then row broadcasts: no LDS round trips).
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1, 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2, 3
+  return v;
+}
+__device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+// ceil(n / size) for 1 <= n, size <= 2^17: the quotient of n - 1/2 is never within rounding of a whole
+// number.
+__device__ __forceinline__ int parts_of(int n, float inv_size) {
+  return n > 0 ? (int)(((float)n - 0.5f) * inv_size) + 1 : 1;
 }
 __device__ __forceinline__ Share find_share(const Params& p, int item, int lane) {
   auto tiles_of = [&](int i) { return i < p.batch ? row_tiles_of(p, row_of(p, i)) : RowTiles{0, 0, 0}; };
@@ -200,30 +211,25 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int lane)
   }
   total = wave_sum(total) * p.num_kv_heads;
   int size = max((total + p.target - 1) / p.target, kMinPart);
+  float inv = 1.f / (float)size;
   for (int step = 0; step < 4; ++step) {
-    int wgs = t0.count * ((t0.n + size - 1) / size);
+    int wgs = t0.count * parts_of(t0.n, inv);
     for (int i0 = 64; i0 < p.batch; i0 += 64) {
       const RowTiles t = tiles_of(i0 + lane);
-      wgs += t.count * ((t.n + size - 1) / size);
+      wgs += t.count * parts_of(t.n, inv);
     }
     wgs = wave_sum(wgs) * p.num_kv_heads;
     if (wgs <= p.target) break;
-    size = max((size * wgs + p.target - 1) / p.target, size + 1);
+    size = max((int)((float)size * (float)wgs / (float)p.target), size + 1);
+    inv = 1.f / (float)size;
   }
-  size = __builtin_amdgcn_readfirstlane(size);
   Share s = {-1, 0, 1};
   int before = 0;
   for (int i0 = 0; i0 < p.batch; i0 += 64) {
     const RowTiles t = i0 == 0 ? t0 : tiles_of(i0 + lane);
-    const int parts = max((t.n + size - 1) / size, 1);
+    const int parts = parts_of(t.n, inv);
     const int items = i0 + lane < p.batch ? t.count * parts + p.row_tiles - t.count : 0;
-    int upto = items;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int x = __shfl_up(upto, d);
-      if (lane >= d) upto += x;
-    }
-    upto += before;
+    const int upto = before + wave_scan(items);
     if (const uint64_t hit = __builtin_amdgcn_ballot_w64(upto > item)) {
       const int l = __builtin_ctzll(hit);
       s.b = i0 + l;
@@ -290,6 +296,17 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The same for LDS only: copies stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+// 16 bits of each wave, as one scalar.
+__device__ __forceinline__ uint64_t uniform64(const uint16_t* x) {
+  const uint64_t v = *(const uint64_t*)x;
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
+         (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+}
+
 // This wave's copies of a tile: K and V of keys 16w .. 16w + 15, whose pool rows (-1: zeros) lanes
 // lane0 .. lane0 + 15 hold in `row`.
 template <int kD>
@@ -317,13 +334,11 @@ struct Slice;
 template <>
 struct Slice<2> {
   typedef half8 frag;
-  typedef unsigned short bits __attribute__((ext_vector_type(8)));
   static __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) { return mfma16x16x32(a, b, c); }
 };
 template <>
 struct Slice<1> {
   typedef half4 frag;
-  typedef unsigned short bits __attribute__((ext_vector_type(4)));
   static __device__ __forceinline__ floatx4 mfma(half4 a, half4 b, floatx4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0);
   }
@@ -421,64 +436,102 @@ __device__ __forceinline__ void pv_read(const typename Slice<kT>::frag (&vf)[kD 
   acc[kD / 16] = Slice<kT>::mfma(splat<kT>(1.f), pf, acc[kD / 16]);
 }
 
-// Whether slice c of V is finite: the product with an all-zero P is NaN where V is not.
-template <int kD, int kT>
-__device__ __forceinline__ bool v_finite(uint32_t vs, int c) {
-  floatx4 chk = {0.f, 0.f, 0.f, 0.f};
+// Infinities and NaN in V.  In the matrix product a value that a row does not see has weight 0, and
+// 0 * inf would reach that row.  Tiles that some row may not see whole are therefore looked over
+// first: each wave those 16 keys of V that it copied (bad_keys, a bit per key).  Where there are
+// any, scrub() replaces such values by zeros and notes them, a bit per column, as +inf (or NaN)
+// and -inf (or NaN); note_row() collects those that a row sees, and mark4() / mark8() put them
+// into its output at the end (both: NaN).  (Put into the accumulators at once they cost the loops
+// their registers.)
+template <int kD>
+struct Notes {
+  uint8_t bit[2][kD / 8];  // of one key or row: +inf or NaN, -inf or NaN
+};
+template <int kD>
+__device__ __forceinline__ uint32_t bad_keys(uint32_t v, int lane) {  // v: V of the wave's keys in LDS
+  typedef u32x4 __attribute__((address_space(3))) * lds_u4;
+  typedef Tile<kD> T;
+  u32x4 x[T::kCopies];
 #pragma unroll
-  for (int dt = 0; dt < kD / 16; ++dt)
-    chk = Slice<kT>::mfma(vt_frag<kD, kT>(vs, c, dt), splat<kT>(0.f), chk);
-  // the file is compiled for NaN-free arithmetic: hide where the bits are from
-  asm volatile("" : "+v"(chk));
-  const u32x4 u = __builtin_bit_cast(u32x4, chk);
-  const uint32_t bad = (u[0] | u[1] | u[2] | u[3]) & 0x7fffffffu;
-  return __builtin_amdgcn_ballot_w64(bad != 0) == 0;
-}
-
-// pv_slice where a key that some rows must not see may hold an infinity or a NaN in V: 0 * inf
-// in the matrix product would reach those rows.  The product runs on V with such values
-// replaced by zeros; then products of indicators (V is +inf or NaN / -inf or NaN; P is not zero)
-// count which of them each row sees, and put the infinities where they belong (both: NaN).
-template <int NB, int kD, int kT>
-__device__ __forceinline__ void pv_slice_careful(uint32_t vs, int c,
-                                                 const typename Slice<kT>::frag (&pf)[NB],
-                                                 floatx4 (&acc)[NB][kD / 16 + 1]) {
-  typedef typename Slice<kT>::bits bits;
-  typedef typename Slice<kT>::frag frag;
-  constexpr int kN = kD / 16;
+  for (int q = 0; q < T::kCopies; ++q) x[q] = *(lds_u4)(v + 1024 * q + 16 * lane);
+  uint32_t bad[T::kCopies], any = 0;
 #pragma unroll
-  for (int dt = 0; dt < kN; ++dt) {
-    const bits v = __builtin_bit_cast(bits, vt_frag<kD, kT>(vs, c, dt));
-    bits ok, inf[2];
+  for (int q = 0; q < T::kCopies; ++q) {
+    bad[q] = 0;
 #pragma unroll
-    for (int e = 0; e < 4 * kT; ++e) {
-      const unsigned short m = v[e] & 0x7fff;
-      ok[e] = m < 0x7c00 ? v[e] : (unsigned short)0;
-      inf[0][e] = m > 0x7c00 || v[e] == 0x7c00 ? (unsigned short)0x3c00 : (unsigned short)0;
-      inf[1][e] = m > 0x7c00 || v[e] == 0xfc00 ? (unsigned short)0x3c00 : (unsigned short)0;
-    }
-#pragma unroll
-    for (int j = 0; j < NB; ++j) {
-      acc[j][dt] = Slice<kT>::mfma(__builtin_bit_cast(frag, ok), pf[j], acc[j][dt]);
-      bits pi = __builtin_bit_cast(bits, pf[j]);
-#pragma unroll
-      for (int e = 0; e < 4 * kT; ++e) pi[e] = pi[e] ? (unsigned short)0x3c00 : (unsigned short)0;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const floatx4 n = Slice<kT>::mfma(__builtin_bit_cast(frag, inf[i]), __builtin_bit_cast(frag, pi),
-                                          floatx4{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = n[r] > 0.f ? (i ? -__builtin_inff() : __builtin_inff()) : 0.f;
-          asm volatile("" : "+v"(x));  // the sum of both infinities has to be taken, not folded
-          acc[j][dt][r] += x;
-        }
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);  // one step's registers at a time
+    for (int e = 0; e < 4; ++e) bad[q] |= (x[q][e] & 0x7c007c00u) + 0x04000400u;  // carries where all ones
+    bad[q] &= 0x80008000u;
+    any |= bad[q];
   }
+  if (__builtin_amdgcn_ballot_w64(any != 0) == 0) return 0;
+  uint32_t keys = 0;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j][kN] = Slice<kT>::mfma(splat<kT>(1.f), pf[j], acc[j][kN]);
+  for (int q = 0; q < T::kCopies; ++q) {
+    const uint64_t m = __builtin_amdgcn_ballot_w64(bad[q] != 0);
+    for (int r = 0; r < T::kCopyRows; ++r)
+      if ((m >> (r * T::kChunks)) & ((1u << T::kChunks) - 1)) keys |= 1u << (q * T::kCopyRows + r);
+  }
+  return keys;
+}
+template <int kD>
+__device__ __forceinline__ void scrub(uint32_t v, Notes<kD>* notes, int lane) {  // notes: of the wave's keys
+  typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+  typedef us8 __attribute__((address_space(3))) * lds_us8;
+  typedef Tile<kD> T;
+  for (int q = 0; q < T::kCopies; ++q) {
+    const lds_us8 at = (lds_us8)(v + 1024 * q + 16 * lane);
+    us8 x = *at;
+    uint32_t up = 0, down = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const unsigned short m = x[e] & 0x7fff;
+      if (m > 0x7c00 || x[e] == 0x7c00) up |= 1u << e;
+      if (m > 0x7c00 || x[e] == 0xfc00) down |= 1u << e;
+      if (m >= 0x7c00) x[e] = 0;
+    }
+    *at = x;
+    const int r = q * T::kCopyRows + lane / T::kChunks, c = (lane % T::kChunks) ^ T::xv(r);
+    notes[r].bit[0][c] = (uint8_t)up;
+    notes[r].bit[1][c] = (uint8_t)down;
+  }
+}
+// Of the keys in `bad` (bit k: key k0 + k), those that a row at `pos` (-1: no token) sees.
+__device__ __forceinline__ uint64_t bad_seen(const Params& p, uint64_t bad, int k0, int prefix, int pos) {
+  uint64_t seen = 0;
+  if (pos < 0) return 0;
+  for (; bad; bad &= bad - 1) {
+    const int k = __builtin_ctzll(bad), key = k0 + k;
+    if (key < prefix || (key <= pos && key > pos - p.window)) seen |= 1ull << k;
+  }
+  return seen;
+}
+template <int kD>
+__device__ __forceinline__ void note_row(const Notes<kD>* keys, uint64_t seen, Notes<kD>* row) {
+  for (; seen; seen &= seen - 1) {
+    const uint32_t* from = (const uint32_t*)&keys[__builtin_ctzll(seen)];
+    for (int i = 0; i < (int)sizeof(Notes<kD>) / 4; ++i) atomicOr((uint32_t*)row + i, from[i]);
+  }
+}
+__device__ __forceinline__ float mark(float x, uint32_t up, uint32_t down) {
+  float a = up ? __builtin_inff() : 0.f, b = down ? -__builtin_inff() : 0.f;
+  // the file is compiled for NaN-free arithmetic: these sums have to be taken, not folded
+  asm volatile("" : "+v"(a), "+v"(b));
+  return (x + a) + b;
+}
+template <int kD>
+__device__ __forceinline__ floatx4 mark4(const Notes<kD>& row, int d, floatx4 v) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    v[r] = mark(v[r], (row.bit[0][(d + r) >> 3] >> ((d + r) & 7)) & 1, (row.bit[1][(d + r) >> 3] >> ((d + r) & 7)) & 1);
+  return v;
+}
+template <int kD>
+__device__ __forceinline__ u32x4 mark8(const Notes<kD>& row, int chunk, u32x4 v) {
+  half8 h = as_half8(v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    h[e] = (half_t)mark((float)h[e], (row.bit[0][chunk] >> e) & 1, (row.bit[1][chunk] >> e) & 1);
+  return as_u32x4(h);
 }
 
 // x = cap_log2 * tanh(y), y = s * sm_scale / cap, in log2 units: tanh(y) = 1 - 2 / (1 + e^2y).
@@ -525,7 +578,7 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
       for (int e = 0; e < kE; ++e) s[j][e >> 2][e & 3] = kMod == kBias ? bias(j, e) : 0.f;
     qk_slice<NB, kD, kT>(ks, c, qf, s);
     frag vf[kD / 16];
-    if constexpr (NB == 1 && !kMasked) {
+    if constexpr (NB == 1) {
 #pragma unroll
       for (int dt = 0; dt < kD / 16; ++dt) vf[dt] = vt_frag<kD, kT>(vs, c, dt);
     }
@@ -598,30 +651,11 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
       for (int e = 0; e < kE; ++e)
         pf[j][e] = (half_t)fast_exp2(__builtin_fmaf(s[j][e >> 2][e & 3], p.scale_log2, -mc));
     }
-    if constexpr (NB == 1 && !kMasked) {
+    if constexpr (NB == 1)
       pv_read<kD, kT>(vf, pf[0], acc[0]);
-    } else {
-      if (kMasked && !v_finite<kD, kT>(vs, c))
-        pv_slice_careful<NB, kD, kT>(vs, c, pf, acc);
-      else
-        pv_slice<NB, kD, kT>(vs, c, pf, acc);
-    }
+    else
+      pv_slice<NB, kD, kT>(vs, c, pf, acc);
   }
-}
-
-// A tile that needs masks, one row block at a time: with all blocks at once the accumulators spill,
-// and the waits for the reloads wait for the next tile's copies too.
-template <int NB, int kD, int kMod, int kT, int kSlices>
-__device__ __forceinline__ void consume_masked(const Params& p, uint32_t ks, uint32_t vs, int k0, uint64_t keys,
-                                               int prefix, const int* s_pos, const float* s_slope, int col,
-                                               int g, const half8 (&qf)[NB][kD / 32], float (&t_run)[NB],
-                                               floatx4 (&acc)[NB][kD / 16 + 1]) {
-#pragma unroll
-  for (int j = 0; j < NB; ++j)
-    consume<1, kD, kMod, kT, kSlices, true>(
-        p, ks, vs, k0, keys, prefix, s_pos + 16 * j, s_slope + (kMod & kBias ? 16 * j : 0), col, g,
-        reinterpret_cast<const half8(&)[1][kD / 32]>(qf[j]), reinterpret_cast<float(&)[1]>(t_run[j]),
-        reinterpret_cast<floatx4(&)[1][kD / 16 + 1]>(acc[j]));
 }
 
 // Q^T fragments of the wave's row blocks, rows r0 on (MFMA i takes d = 32 i + 8 g + s in reduction
@@ -703,7 +737,9 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   __shared__ int s_pos[kRows];  // position of each query row, -1 for rows without a token
   __shared__ float s_slope[kMod & kBias ? kRows : 1];  // its distance bias in score units
   __shared__ int s_ent[4][kWaves][64];
-  __shared__ __attribute__((aligned(8))) uint16_t s_keys[2][kWaves];
+  __shared__ __attribute__((aligned(8))) uint16_t s_keys[2][kWaves], s_bad[kWaves];
+  __shared__ Notes<kD> s_notes[kKTile];    // of the keys of a tile,
+  __shared__ Notes<kD> s_rows[kRows];      // of the rows, where `noted`
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -765,23 +801,39 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   // Tile i lies in stage i % 2.  While it is consumed, tile i + 1 is copied into the other stage
   // (whose readers have passed the last barrier).
   auto copy_next = [&](int i) -> uint64_t {  // the keys of tile i
-    const uint64_t k = *(const uint64_t*)s_keys[i & 1];
+    const uint64_t keys = uniform64(s_keys[i & 1]);
     if (i > 0) {  // the first two are on their way
       copy_entries(i + 3);
       copy_tile(i + 1);
     }
-    return ((uint64_t)__builtin_amdgcn_readfirstlane((int)(k >> 32)) << 32) |
-           (uint32_t)__builtin_amdgcn_readfirstlane((int)k);
+    return keys;
   };
   const uint32_t ks = lds_addr(stages) + k_lane<kD>(col, g);
   const uint32_t vs = lds_addr(stages) + T::kBytes + v_lane<kD>(col, g);
   int i = 0;
+  const uint32_t v_own = lds_addr(stages) + T::kBytes + 16 * w * T::kRow;  // V of the keys it copies
+  bool noted = false;
   for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
     const uint64_t keys = copy_next(i);
+    const int at = (i & 1) * T::kStage;
+    const uint32_t mine = bad_keys<kD>(v_own + at, lane);
+    if (lane == 0) s_bad[w] = (uint16_t)mine;
+    lds_barrier();
+    const uint64_t bad = uniform64(s_bad);
     const int k0 = span.tile(first + i) * kKTile;
+    if (bad) {
+      scrub<kD>(v_own + at, s_notes + 16 * w, lane);
+      lds_barrier();
+      if (lane < kRowsPerWave) {
+        Notes<kD>& r = s_rows[kRowsPerWave * w + lane];
+        if (!noted) r = Notes<kD>{};
+        note_row<kD>(s_notes, bad_seen(p, bad & keys, k0, row.prefix, w_pos[lane]), &r);
+      }
+      noted = true;
+    }
     if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
-      consume_masked<NB, kD, kMod, 2, 2>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage, k0, keys,
-                                        row.prefix, w_pos, w_slope, col, g, qf, t_run, acc);
+      consume<NB, kD, kMod, 2, 2, true>(p, ks + at, vs + at, k0, keys, row.prefix, w_pos, w_slope, col, g, qf,
+                                        t_run, acc);
     stage_barrier();
   }
   for (; i < n; ++i) {
@@ -800,7 +852,11 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
       if (w_pos[16 * j + col] < 0) continue;
       const int64_t slot = (int64_t)blockIdx.x * p.part_rows + rl;
 #pragma unroll
-      for (int dt = 0; dt < kD / 16; ++dt) *(floatx4*)(p.part_o + slot * kD + 16 * dt + 4 * g) = acc[j][dt];
+      for (int dt = 0; dt < kD / 16; ++dt) {
+        floatx4 v = acc[j][dt];
+        if (noted) v = mark4<kD>(s_rows[rl], 16 * dt + 4 * g, v);
+        *(floatx4*)(p.part_o + slot * kD + 16 * dt + 4 * g) = v;
+      }
       if (g == 0) {
         p.part_ml[slot * 2] = __builtin_fmaf(t_run[j], p.scale_log2, -p.lazy_log2);
         p.part_ml[slot * 2 + 1] = acc[j][kD / 16][0];
@@ -831,7 +887,8 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     const int r = r0 + kRowsPerWave * w + rl;
     const int t = div_by(r, p.group_div);
     const int h = kvh * p.group + r - t * p.group;
-    const u32x4 v = *(const u32x4*)(ostage + rl * kORow + 16 * oc);
+    u32x4 v = *(const u32x4*)(ostage + rl * kORow + 16 * oc);
+    if (noted) v = mark8<kD>(s_rows[kRowsPerWave * w + rl], oc, v);
     if (t < p.chunk && oc < p.d_chunks)
       *(u32x4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + 8 * oc) = v;
   }
@@ -853,6 +910,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
   __shared__ int s_pos[kWaves][kRows];
   __shared__ float s_slope[kWaves][kMod & kBias ? kRows : 1];
   __shared__ float s_ml[kWaves][kRows][2];
+  __shared__ Notes<kD> s_notes[kWaves][16];  // of the keys of a wave's tile,
+  __shared__ Notes<kD> s_rows[kRows];        // of the rows, where s_noted
+  __shared__ int s_noted;
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -889,6 +949,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
   for (int i = 0; i < 3; ++i) copy_entries(i);
   half8 qf[NB][kD / 32];
   load_rows<NB, kD, kMod>(p, row, b, kvh, r0, col, g, qf, s_pos[w], s_slope[w]);
+  if (tid < kRows) s_rows[tid] = Notes<kD>{};
+  if (tid == 0) s_noted = 0;
+  lds_barrier();
   // also for the compiler, which would otherwise wait for every copy at the first use of Q
   wait_vmcnt<0>();
   asm volatile("" ::: "memory");
@@ -925,11 +988,22 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
     }
   };
   int i = 0;
+  const uint32_t v_own = lds_addr(stages) + T::kBytes + 16 * w * T::kRow;
   for (const int end = min(max(span.masked() - first, 0), n); i < end; ++i) {
     arrive(i);
-    consume_masked<NB, kD, kMod, 1, 1>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
-                                      span.tile(first + i) * kKTile + 16 * w, keys, row.prefix, s_pos[w],
-                                      s_slope[w], col, g, qf, t_run, acc);
+    const int at = (i & 1) * T::kStage;
+    const int k0 = span.tile(first + i) * kKTile + 16 * w;
+    const uint32_t bad = bad_keys<kD>(v_own + at, lane);
+    if (bad) {
+      scrub<kD>(v_own + at, s_notes[w], lane);
+      wave_lds_sync();
+      if (lane < kRows)
+        note_row<kD>(s_notes[w], bad_seen(p, bad & keys, k0, row.prefix, s_pos[w][lane]), &s_rows[lane]);
+      if (lane == 0) s_noted = 1;
+      wave_lds_sync();
+    }
+    consume<NB, kD, kMod, 1, 1, true>(p, ks + at, vs + at, k0, keys, row.prefix, s_pos[w], s_slope[w], col, g,
+                                      qf, t_run, acc);
     advance(i);
   }
   for (; i < n; ++i) {
@@ -977,6 +1051,7 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
         l += lw * e;
         o += *(const floatx4*)(cmb + (ww * 16 + c) * kD + d) * e;
       }
+      if (s_noted) o = mark4<kD>(s_rows[rl], d, o);
       const bool there = s_pos[0][rl] >= 0;
       if (job.parts > 1) {
         if (!there) continue;

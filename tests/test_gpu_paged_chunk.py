@@ -433,3 +433,30 @@ def test_many_rows_share_the_work_list(hip):
     starts = [n - int(c) for n, c in zip(lens, torch.randint(0, new + 1, (batch,), generator=g))]
     q, kc, vc, table = _case(24, lens, new, 3, 1, 64, 16)
     _check(q, kc, vc, table, 16, lens, starts)
+
+
+@pytest.mark.parametrize("new", [1, 5, 9, 60])
+def test_infinite_values_per_column_padding_and_parts(hip, new):
+    """Single infinite columns in the chunk, in the prefix and past the window, on a padded batch
+    whose context is cut into parts: rows that see them, and padding, which stays zero."""
+    banner(f"chunk attention infinite columns, {new} new")
+    import fast_infer_amd as fi
+
+    lens, bs, window, prefix = [2000, 700], 16, 100, [70, 3]
+    starts = [2000 - new, 700 - (new + 1) // 2]
+    q, kc, vc, table = _case(25, lens, new, 6, 2, 128, bs)
+    want, bound = OC.chunk_attention(q, kc, vc, table, bs, lens, starts, window=window, prefix=prefix)
+    spots = [(0, 69, 0, 3), (0, 70, 0, 4), (0, 1999, 1, 127), (0, 1900 - new, 1, 64), (1, 2, 0, 9), (1, 699, 1, 31)]
+    for b, pos, h, c in spots:
+        vc[table[b, pos // bs].long(), pos % bs, h, c] = math.inf if pos % 2 else -math.inf
+    out = fi.paged_chunk_attention(q, kc, vc, table, bs, 2000, start_positions=_i32(starts),
+                                   context_lens=_i32(lens), window=window, prefix_lens=_i32(prefix))
+    for b, pos, h, c in spots:
+        for t in range(new):
+            at = starts[b] + t
+            if at < lens[b] and (pos < prefix[b] or at - window < pos <= at):
+                want[b, t, 3 * h:3 * h + 3, c] = math.inf if pos % 2 else -math.inf
+    finite = torch.isfinite(want)
+    assert torch.equal(out.double()[~finite], want[~finite])
+    assert ((out.double() - want).abs() <= bound)[finite].all()
+    assert not out[1, (new + 1) // 2:].any()
