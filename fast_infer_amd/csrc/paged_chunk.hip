@@ -202,6 +202,12 @@ __device__ __forceinline__ int parts_of(int n, float inv_size) {
   return n > 0 ? (int)(((float)n - 0.5f) * inv_size) + 1 : 1;
 }
 __device__ __forceinline__ Share find_share(const Params& p, int item, int lane) {
+  if (p.batch == 1) {
+    const RowTiles t = row_tiles_of(p, row_of(p, 0));
+    const int most = max(p.target / max(t.count * p.num_kv_heads, 1), 1);  // parts in one round
+    const int parts = max(min(most, (t.n + kMinPart - 1) / kMinPart), 1);
+    return {item < t.count * parts + p.row_tiles - t.count ? 0 : -1, 0, parts};
+  }
   auto tiles_of = [&](int i) { return i < p.batch ? row_tiles_of(p, row_of(p, i)) : RowTiles{0, 0, 0}; };
   const RowTiles t0 = tiles_of(lane);
   int total = t0.count * t0.n;
@@ -278,6 +284,13 @@ __device__ __forceinline__ void lds_copy16_global(const char* src, uint32_t lds)
                : "memory");
 }
 
+// The same with the non-temporal policy, for keys that one workgroup reads.
+__device__ __forceinline__ void lds_copy16_global_nt(const char* src, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
+               :
+               : "s"(lds), "v"(src)
+               : "memory");
+}
 // The same with 4 bytes a lane.
 __device__ __forceinline__ void lds_copy4_global(const int32_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
@@ -309,7 +322,7 @@ __device__ __forceinline__ uint64_t uniform64(const uint16_t* x) {
 
 // This wave's copies of a tile: K and V of keys 16w .. 16w + 15, whose pool rows (-1: zeros) lanes
 // lane0 .. lane0 + 15 hold in `row`.
-template <int kD>
+template <int kD, bool kOnce>
 __device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, const char* vbase,
                                            char* stage, int row, int lane0, int w, int lane) {
   typedef Tile<kD> T;
@@ -321,9 +334,15 @@ __device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, c
     const int from = __shfl(row, lane0 + r);
     const int64_t at = from * p.row_bytes;
     const int kc = slot ^ T::xk(r), vc = slot ^ T::xv(r);
-    lds_copy16_global((from >= 0 && kc < p.d_chunks ? kbase + at : g_zeros) + 16 * kc, dst + 1024 * q);
-    lds_copy16_global((from >= 0 && vc < p.d_chunks ? vbase + at : g_zeros) + 16 * vc,
-                      dst + T::kBytes + 1024 * q);
+    const char* ks = (from >= 0 && kc < p.d_chunks ? kbase + at : g_zeros) + 16 * kc;
+    const char* vs = (from >= 0 && vc < p.d_chunks ? vbase + at : g_zeros) + 16 * vc;
+    if (kOnce) {
+      lds_copy16_global_nt(ks, dst + 1024 * q);
+      lds_copy16_global_nt(vs, dst + T::kBytes + 1024 * q);
+    } else {
+      lds_copy16_global(ks, dst + 1024 * q);
+      lds_copy16_global(vs, dst + T::kBytes + 1024 * q);
+    }
   }
 }
 
@@ -602,13 +621,15 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
     if (kMasked) {
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
-        const int pos = s_pos[16 * j + col];
+        // without branches: as conditions they took three times a full tile's time
+        const int back = s_pos[16 * j + col] - key0, ahead = prefix - key0;
+        const uint32_t here = (uint32_t)(keys >> (16 * kT * c)) >> (4 * g);
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
-          const int key = key0 + 16 * (e >> 2) + (e & 3);
-          const bool see = (key < prefix || (key <= pos && key > pos - p.window)) &&
-                           ((keys >> (key - k0)) & 1);
-          if (!see) s[j][e >> 2][e & 3] = -__builtin_inff();
+          const int at = 16 * (e >> 2) + (e & 3);
+          const bool see = (((uint32_t)(back - at) < (uint32_t)p.window) | (ahead > at)) &
+                           (((here >> at) & 1) != 0);
+          s[j][e >> 2][e & 3] = see ? s[j][e >> 2][e & 3] : -__builtin_inff();
         }
       }
     } else if (keys != kAll) {  // missing table entries
@@ -772,15 +793,11 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
     const int at = entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
     const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
     if (lane == 0) s_keys[i & 1][w] = (uint16_t)there;
-    issue_tile<kD>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
+    issue_tile<kD, false>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
   };
 
 #pragma unroll
   for (int i = 0; i < 3; ++i) copy_entries(i);
-  half8 qf[NB][kD / 32];
-  int* w_pos = s_pos + kRowsPerWave * w;
-  float* w_slope = s_slope + (kMod & kBias ? kRowsPerWave * w : 0);
-  load_rows<NB, kD, kMod>(p, row, b, kvh, r0 + kRowsPerWave * w, col, g, qf, w_pos, w_slope);
   int wlo, whi;  // positions of this wave's tokens
   row_positions(p, row, r0 + kRowsPerWave * w, r0 + kRowsPerWave * (w + 1) - 1, wlo, whi);
 
@@ -796,6 +813,10 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   copy_tile(0);
   copy_entries(3);
   copy_tile(1);
+  half8 qf[NB][kD / 32];
+  int* w_pos = s_pos + kRowsPerWave * w;
+  float* w_slope = s_slope + (kMod & kBias ? kRowsPerWave * w : 0);
+  load_rows<NB, kD, kMod>(p, row, b, kvh, r0 + kRowsPerWave * w, col, g, qf, w_pos, w_slope);
   stage_barrier();
 
   // Tile i lies in stage i % 2.  While it is consumed, tile i + 1 is copied into the other stage
@@ -941,26 +962,27 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
     const int slot = key - div_by(key, p.block_div) * p.block_size;
     const int entry = s_ent[w][i & (kEnts - 1)][lane];
     const int at = entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
-    issue_tile<kD>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
+    issue_tile<kD, true>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
     return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0) & 0xffffu;
   };
 
 #pragma unroll
   for (int i = 0; i < 3; ++i) copy_entries(i);
-  half8 qf[NB][kD / 32];
-  load_rows<NB, kD, kMod>(p, row, b, kvh, r0, col, g, qf, s_pos[w], s_slope[w]);
-  if (tid < kRows) s_rows[tid] = Notes<kD>{};
-  if (tid == 0) s_noted = 0;
-  lds_barrier();
-  // also for the compiler, which would otherwise wait for every copy at the first use of Q
-  wait_vmcnt<0>();
-  asm volatile("" ::: "memory");
+  wait_copies<0>();
   uint32_t keys = 0, keys_next = 0;
   if (n > 0) keys = copy_tile(0);
   if (n > 1) {
     copy_entries(3);
     keys_next = copy_tile(1);
   }
+  half8 qf[NB][kD / 32];
+  load_rows<NB, kD, kMod>(p, row, b, kvh, r0, col, g, qf, s_pos[w], s_slope[w]);
+  if (tid < kRows) s_rows[tid] = Notes<kD>{};
+  if (tid == 0) s_noted = 0;
+  // Q and the first tiles have landed, also for the compiler, which would otherwise wait for every
+  // copy at the first use of Q
+  wait_vmcnt<0>();
+  lds_barrier();
 
   float t_run[NB];
   floatx4 acc[NB][kD / 16 + 1];
