@@ -64,6 +64,7 @@ struct Params {
   const half_t* v_cache;
   int num_pool_blocks;
   int block_size;
+  int whole;  // block_size % 16 == 0: the 16 keys that a wave copies lie in one block
   FastDiv block_div;
   int num_kv_heads;
   int64_t row_bytes;  // one pool slot, all kv heads
@@ -291,6 +292,20 @@ __device__ __forceinline__ void lds_copy16_global_nt(const char* src, uint32_t l
                : "s"(lds), "v"(src)
                : "memory");
 }
+// The same from a common base and 32-bit offsets.
+template <bool kOnce>
+__device__ __forceinline__ void lds_copy16_base(const char* base, uint32_t offset, uint32_t lds) {
+  if (kOnce)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
+                 :
+                 : "s"(lds), "v"(offset), "s"(base)
+                 : "memory");
+  else
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+                 :
+                 : "s"(lds), "v"(offset), "s"(base)
+                 : "memory");
+}
 // The same with 4 bytes a lane.
 __device__ __forceinline__ void lds_copy4_global(const int32_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
@@ -345,6 +360,96 @@ __device__ __forceinline__ void issue_tile(const Params& p, const char* kbase, c
     }
   }
 }
+
+// The copies of one wave: keys 16w .. 16w + 15 of the part's tiles, and the table entries they need.
+// Entries come through LDS (s_ent, 256 of the wave): an ordinary load in the loop would make the
+// compiler wait for every copy.  Blocks of a multiple of 16 tokens: one entry a tile, those of 64
+// tiles a copy; then the copies of a tile of 16 valid keys take a scalar base and constant
+// offsets (with an address per lane the wide kernel spends a third of its vector instructions on
+// them).  Other sizes: an entry per key, lane l's for key l % 16, copied two tiles ahead of the keys'.
+template <int kD, bool kOnce>
+struct Copier {
+  typedef Tile<kD> T;
+  const Params& p;
+  const Span& span;
+  int first, n, len, w, lane;
+  const int32_t* table;
+  const char *kbase, *vbase;
+  char* stages;
+  int* s_ent;
+  uint32_t k_off, v_off;
+
+  __device__ __forceinline__ Copier(const Params& p_, const Span& span_, int first_, int n_, int len_, int b,
+                                    int kvh, int w_, int lane_, char* stages_, int* s_ent_)
+      : p(p_), span(span_), first(first_), n(n_), len(len_), w(w_), lane(lane_),
+        table(p_.block_table + (int64_t)b * p_.bt_stride),
+        kbase((const char*)(p_.k_cache + (int64_t)kvh * p_.head_dim)),
+        vbase((const char*)(p_.v_cache + (int64_t)kvh * p_.head_dim)), stages(stages_), s_ent(s_ent_) {
+    const int r = lane / T::kChunks;
+    const uint32_t row = (uint32_t)(r * (int)p.row_bytes);
+    k_off = row + 16 * ((lane % T::kChunks) ^ T::xk(r));
+    v_off = row + 16 * ((lane % T::kChunks) ^ T::xv(r));
+  }
+  __device__ __forceinline__ int key_of(int i) const { return span.tile(first + i) * kKTile + 16 * w; }
+  __device__ __forceinline__ void entry(int i, int more, int slot) const {  // of key key_of(i) + more
+    const int key = key_of(i) + more;
+    const int blk = div_by(key, p.block_div);
+    lds_copy4_global(i < n && key < len && blk < p.max_blocks_per_seq ? table + blk : &g_no_block,
+                     lds_addr(s_ent + slot));
+  }
+  // The entries before the first tile, and with tile i (then those of tile i + 4 or of the next 64).
+  __device__ __forceinline__ void first_entries() const {
+    if (p.whole) {
+      entry(lane, 0, 0);
+      if (n > 64) entry(64 + lane, 0, 64);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) entry(i, lane & 15, 64 * i);
+    }
+  }
+  __device__ __forceinline__ void more_entries(int i) const {
+    if (!p.whole)
+      entry(i + 4, lane & 15, 64 * (i & 3));
+    else if (i > 0 && (i & 63) == 0)
+      entry(i + 64 + lane, 0, (i + 64) & 64);
+  }
+  // The copies of tile i; returns its keys in the pool, one bit each.
+  __device__ __forceinline__ uint32_t tile(int i) const {
+    char* stage = stages + (i & 1) * T::kStage;
+    const int key = key_of(i);
+    int at;
+    if (p.whole) {
+      const int e = __builtin_amdgcn_readfirstlane(s_ent[i & 127]);
+      const int slot = key - div_by(key, p.block_div) * p.block_size;
+      const int valid = e >= 0 && e < p.num_pool_blocks ? min(len - key, 16) : 0;
+      const int64_t row = (int64_t)e * p.block_size + slot;
+      if (valid == 16 && p.d_chunks == T::kChunks) {
+        const char* kb = kbase + row * p.row_bytes;
+        const char* vb = vbase + row * p.row_bytes;
+        const uint32_t dst = lds_addr(stage) + 16 * w * T::kRow;
+#pragma unroll
+        for (int q = 0; q < T::kCopies; ++q) {
+          // rows 4 on of every 8: the other half of the permutation (head_dim is kD: a row is a
+          // multiple of 256 bytes)
+          const bool odd = kD == 128 && (q & 1);
+          lds_copy16_base<kOnce>(kb, odd ? k_off ^ 32 : k_off, dst + 1024 * q);
+          lds_copy16_base<kOnce>(vb, odd ? v_off ^ 128 : v_off, dst + T::kBytes + 1024 * q);
+          kb += T::kCopyRows * p.row_bytes;
+          vb += T::kCopyRows * p.row_bytes;
+        }
+        return 0xffffu;
+      }
+      at = (lane & 15) < valid ? (int)row + (lane & 15) : -1;
+    } else {
+      const int mine = key + (lane & 15);
+      const int slot = mine - div_by(mine, p.block_div) * p.block_size;
+      const int e = s_ent[64 * (i & 3) + lane];
+      at = e >= 0 && e < p.num_pool_blocks ? e * p.block_size + slot : -1;
+    }
+    issue_tile<kD, kOnce>(p, kbase, vbase, stage, at, 0, w, lane);
+    return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0) & 0xffffu;
+  }
+};
 
 // A slice of 16 kT keys (kT = 2 or 1) is what one step of the softmax covers.  P and V^T fragments
 // hold 4 kT keys a lane: with kT = 2 keys 4g + j and 16 + 4g + j (j = 0..3) in slots j and 4 + j.
@@ -757,7 +862,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
   __shared__ int s_pos[kRows];  // position of each query row, -1 for rows without a token
   __shared__ float s_slope[kMod & kBias ? kRows : 1];  // its distance bias in score units
-  __shared__ int s_ent[4][kWaves][64];
+  __shared__ int s_ent[kWaves][256];
   __shared__ __attribute__((aligned(8))) uint16_t s_keys[2][kWaves], s_bad[kWaves];
   __shared__ Notes<kD> s_notes[kKTile];    // of the keys of a tile,
   __shared__ Notes<kD> s_rows[kRows];      // of the rows, where `noted`
@@ -773,31 +878,12 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const Row& row = job.row;
   const Span& span = job.span;
 
-  // Lane l of wave w holds the table entry, then the pool row, of key 16w + l % 16 of a tile; the
-  // entries come through LDS: an ordinary load in the loop would make the compiler wait for every
-  // copy.  Their copies run two tiles ahead of the keys'.
-  auto key_of = [&](int i) { return span.tile(first + i) * kKTile + 16 * w + col; };
-  auto copy_entries = [&](int i) {
-    const int key = key_of(i);
-    const int blk = div_by(key, p.block_div);
-    const int32_t* src = i < n && key < row.len && blk < p.max_blocks_per_seq
-                             ? p.block_table + (int64_t)b * p.bt_stride + blk : &g_no_block;
-    lds_copy4_global(src, lds_addr(&s_ent[i & 3][w][0]));
-  };
-  const char* kbase = (const char*)(p.k_cache + (int64_t)kvh * p.head_dim);
-  const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
-  auto copy_tile = [&](int i) {  // with its keys in the pool, 16 bits a wave
-    const int key = key_of(i);
-    const int slot = key - div_by(key, p.block_div) * p.block_size;
-    const int entry = s_ent[i & 3][w][lane];
-    const int at = entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
-    const uint32_t there = (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0);
+  const Copier<kD, false> copies(p, span, first, n, row.len, b, kvh, w, lane, stages, s_ent[w]);
+  auto copy_tile = [&](int i) {
+    const uint32_t there = copies.tile(i);
     if (lane == 0) s_keys[i & 1][w] = (uint16_t)there;
-    issue_tile<kD, false>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
   };
-
-#pragma unroll
-  for (int i = 0; i < 3; ++i) copy_entries(i);
+  copies.first_entries();
   int wlo, whi;  // positions of this wave's tokens
   row_positions(p, row, r0 + kRowsPerWave * w, r0 + kRowsPerWave * (w + 1) - 1, wlo, whi);
 
@@ -811,7 +897,6 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   }
   wait_copies<0>();
   copy_tile(0);
-  copy_entries(3);
   copy_tile(1);
   half8 qf[NB][kD / 32];
   int* w_pos = s_pos + kRowsPerWave * w;
@@ -823,10 +908,8 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   // (whose readers have passed the last barrier).
   auto copy_next = [&](int i) -> uint64_t {  // the keys of tile i
     const uint64_t keys = uniform64(s_keys[i & 1]);
-    if (i > 0) {  // the first two are on their way
-      copy_entries(i + 3);
-      copy_tile(i + 1);
-    }
+    copies.more_entries(i);
+    if (i > 0) copy_tile(i + 1);  // the first two are on their way
     return keys;
   };
   const uint32_t ks = lds_addr(stages) + k_lane<kD>(col, g);
@@ -918,16 +1001,13 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
 // Few rows (at most 16 NB): every wave has all of them and takes 16 keys of each tile, those that it
 // copies itself, so the waves run without barriers, each waiting for its own copies only, and
 // are added up through LDS at the end.  Bound by the stream of K and V: with the rows of one
-// wave and shared tiles, 2.9 TB/s.  The table entries come through LDS as well (an ordinary load
-// in the loop would make the compiler wait for every copy): their copies run two tiles ahead of
-// the keys' copies, which run one tile ahead of the sums.
+// wave and shared tiles, 2.9 TB/s.
 template <int NB, int kD, int kMod>
 __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_kernel(Params p) {
   typedef Tile<kD> T;
   constexpr int kRows = 16 * NB;
-  constexpr int kEnts = 4;
   __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
-  __shared__ int s_ent[kWaves][kEnts][64];
+  __shared__ int s_ent[kWaves][256];
   __shared__ int s_pos[kWaves][kRows];
   __shared__ float s_slope[kWaves][kMod & kBias ? kRows : 1];
   __shared__ float s_ml[kWaves][kRows][2];
@@ -946,35 +1026,12 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
   const Row& row = job.row;
   const Span& span = job.span;
 
-  // Lane l stands for key 16w + l % 16 of a tile.
-  auto key_of = [&](int i) { return span.tile(first + i) * kKTile + 16 * w + col; };
-  auto copy_entries = [&](int i) {
-    const int key = key_of(i);
-    const int blk = div_by(key, p.block_div);
-    const int32_t* src = i < n && key < row.len && blk < p.max_blocks_per_seq
-                             ? p.block_table + (int64_t)b * p.bt_stride + blk : &g_no_block;
-    lds_copy4_global(src, lds_addr(&s_ent[w][i & (kEnts - 1)][0]));
-  };
-  const char* kbase = (const char*)(p.k_cache + (int64_t)kvh * p.head_dim);
-  const char* vbase = (const char*)(p.v_cache + (int64_t)kvh * p.head_dim);
-  auto copy_tile = [&](int i) -> uint32_t {  // its keys in the pool, one bit each
-    const int key = key_of(i);
-    const int slot = key - div_by(key, p.block_div) * p.block_size;
-    const int entry = s_ent[w][i & (kEnts - 1)][lane];
-    const int at = entry >= 0 && entry < p.num_pool_blocks ? entry * p.block_size + slot : -1;
-    issue_tile<kD, true>(p, kbase, vbase, stages + (i & 1) * T::kStage, at, 0, w, lane);
-    return (uint32_t)__builtin_amdgcn_ballot_w64(at >= 0) & 0xffffu;
-  };
-
-#pragma unroll
-  for (int i = 0; i < 3; ++i) copy_entries(i);
+  const Copier<kD, true> copies(p, span, first, n, row.len, b, kvh, w, lane, stages, s_ent[w]);
+  copies.first_entries();
   wait_copies<0>();
   uint32_t keys = 0, keys_next = 0;
-  if (n > 0) keys = copy_tile(0);
-  if (n > 1) {
-    copy_entries(3);
-    keys_next = copy_tile(1);
-  }
+  if (n > 0) keys = copies.tile(0);
+  if (n > 1) keys_next = copies.tile(1);
   half8 qf[NB][kD / 32];
   load_rows<NB, kD, kMod>(p, row, b, kvh, r0, col, g, qf, s_pos[w], s_slope[w]);
   if (tid < kRows) s_rows[tid] = Notes<kD>{};
@@ -994,10 +1051,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
   }
   const uint32_t ks = lds_addr(stages) + 16 * w * T::kRow + k_lane<kD>(col, g);
   const uint32_t vs = lds_addr(stages) + T::kBytes + 16 * w * T::kRow + v_lane<kD>(col, g);
-  // behind tile i: the entries of tile i + 3 and tile i + 1 are on their way
-  auto arrive = [&](int i) {
+  auto arrive = [&](int i) {  // tile i; tile i + 1 is on its way
     if (i + 1 < n)
-      wait_copies<2 * T::kCopies + 1>();
+      wait_copies<2 * T::kCopies>();
     else
       wait_copies<0>();
   };
@@ -1005,8 +1061,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
     keys = keys_next;
     if (i + 2 < n) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the reads of this stage are done
-      copy_entries(i + 4);
-      keys_next = copy_tile(i + 2);
+      copies.more_entries(i);
+      keys_next = copies.tile(i + 2);
     }
   };
   int i = 0;
@@ -1037,8 +1093,10 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
   }
 
   // Add the waves up, one row block at a time: O and the sums relative to the waves' own maxima.
-  float* cmb = (float*)stages;  // [wave][16][kD]
-  static_assert(kWaves * 16 * kD * 4 <= 2 * T::kStage, "a row block of every wave fits the stages");
+  // (Rows padded by 16 bytes: the 16 rows of one write would share a bank.)
+  constexpr int kPad = kD + 4;
+  float* cmb = (float*)stages;  // [wave][16][kPad]
+  static_assert(kWaves * 16 * kPad * 4 <= 2 * T::kStage, "a row block of every wave fits the stages");
   if (g == 0) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
@@ -1052,7 +1110,7 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
     __syncthreads();
 #pragma unroll
     for (int dt = 0; dt < kD / 16; ++dt)
-      *(floatx4*)(cmb + (w * 16 + col) * kD + 16 * dt + 4 * g) = acc[j][dt];
+      *(floatx4*)(cmb + (w * 16 + col) * kPad + 16 * dt + 4 * g) = acc[j][dt];
     __syncthreads();
     for (int x = tid; x < 16 * kD / 4; x += kThreads) {
       const int c = x / (kD / 4), d = x % (kD / 4) * 4;
@@ -1071,7 +1129,7 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
         if (__builtin_bit_cast(uint32_t, lw) == 0) continue;  // saw no key (a NaN is not 0)
         const float e = fast_exp2(s_ml[ww][rl][0] - m);
         l += lw * e;
-        o += *(const floatx4*)(cmb + (ww * 16 + c) * kD + d) * e;
+        o += *(const floatx4*)(cmb + (ww * 16 + c) * kPad + d) * e;
       }
       if (s_noted) o = mark4<kD>(s_rows[rl], d, o);
       const bool there = s_pos[0][rl] >= 0;
@@ -1270,7 +1328,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
   }
   if (batch == 0 || num_new == 0) return FI_OK;
   if (num_tokens > kMaxTokens || num_pool_blocks > 0x7fffffff / block_size ||
-      max_blocks_per_seq > 0x7fffffff || batch > 0x7fffffff / num_kv_heads ||
+      max_blocks_per_seq > 0x7fffffff || batch > 0x7fffffff / num_kv_heads || num_kv_heads > (1 << 19) ||
       num_new > 0x7fffffff / num_q_heads / 2) {
     set_error("%s: sizes too large (at most %lld tokens a row, 2^31 pool slots)", fn,
               (long long)kMaxTokens);
@@ -1294,6 +1352,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.v_cache = (const half_t*)v_cache;
   p.num_pool_blocks = (int)num_pool_blocks;
   p.block_size = (int)block_size;
+  p.whole = block_size % 16 == 0;
   p.block_div = fast_div((uint32_t)block_size);
   p.num_kv_heads = (int)num_kv_heads;
   p.row_bytes = num_kv_heads * head_dim * 2;

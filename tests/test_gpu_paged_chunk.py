@@ -460,3 +460,26 @@ def test_infinite_values_per_column_padding_and_parts(hip, new):
     assert torch.equal(out.double()[~finite], want[~finite])
     assert ((out.double() - want).abs() <= bound)[finite].all()
     assert not out[1, (new + 1) // 2:].any()
+
+
+@pytest.mark.parametrize("bs", [8, 16, 24])
+@pytest.mark.parametrize("new", [2, 50])
+def test_long_parts(hip, bs, new):
+    """Parts of far more than 64 key tiles (no workspace): entries in the pool and missing ones
+    throughout, block sizes with one entry per 16 keys and with several."""
+    banner(f"chunk attention long parts, block size {bs}, {new} new")
+    from fast_infer_amd import _lib
+
+    n = 17_003
+    q, kc, vc, table = _case(26, [n], new, 6, 2, 64, bs)
+    gone = torch.randperm(table.shape[1], generator=torch.Generator().manual_seed(1))[:40]
+    table[0, gone.to(DEV)] = -1
+    exact, bound = OC.chunk_attention(q, kc, vc, table, bs, [n])
+    o = torch.empty_like(q)
+    rc = _lib.load().fi_paged_chunk_attention_fwd(
+        q.data_ptr(), *q.stride()[:3], kc.data_ptr(), vc.data_ptr(), kc.shape[0], bs, 2,
+        table.data_ptr(), table.stride(0), table.shape[1], None, None, n, o.data_ptr(), *o.stride()[:3],
+        1, new, 6, 64, 0.125, 0.0, None, 0, None, None, 0, torch.cuda.current_stream().cuda_stream)
+    assert rc == 0
+    ok, msg = OC.is_close(o, exact, bound)
+    assert ok, msg
