@@ -23,6 +23,7 @@
 //     length, on the device; the parts' unnormalised results are added by a second kernel.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "common.h"
 
@@ -96,7 +97,8 @@ struct Params {
   int tile_rows;      // query rows of a row tile, 64 * NB
   FastDiv tile_div;
   int row_tiles;      // of each (batch row, kv head): ceil(chunk * group / tile_rows)
-  int target;         // parts aimed at, all kv heads together
+  int target;         // parts aimed at, all kv heads together: one round of workgroups
+  int target2;        // or this many, where one round would be uneven (0: never)
   int part_rows;      // min(tile_rows, chunk * group): rows of a part's results
   float* part_o;      // [parts, num_kv_heads][part_rows][128]; null: no parts, write o
   float* part_ml;     // [...][2]: reference max (log2 units), sum
@@ -149,6 +151,7 @@ __device__ __forceinline__ Span span_of(const Params& p, const Row& row, int lo,
   const int end = max((hi + kKTile) / kKTile, s.from);
   s.n = s.n_pre + end - s.from;
   s.full_pre = row.prefix / kKTile;
+  if (p.slopes) s.full_pre = min(s.full_pre, (lo + 1) / kKTile);  // the distance bias bends at the row
   // causal tiles that every row sees whole: behind hi - window, and up to lo
   const int a = min(max(hi >= p.window ? (hi - p.window) / kKTile + 1 : 0, s.from), end);
   const int e = max(min((lo + 1) / kKTile, end), a);
@@ -177,11 +180,15 @@ __device__ __forceinline__ RowTiles row_tiles_of(const Params& p, const Row& row
 }
 
 // Every workgroup finds its part by itself, from the lengths on the device: each row tile of batch
-// row b is cut into parts(b) = ceil(its longest list / size) equal pieces, with the size at which
-// about `target` parts, what the device holds at once, take all key tiles (a few steps from below;
-// one more round of workgroups, however few, takes as long as the first); the work list is, for
+// row b is cut into parts(b) = ceil(its longest list / size) equal pieces; the work list is, for
 // each b, its parts (row tile fastest, so that neighbours read the same keys), then its row
-// tiles without tokens, one each.  The batch row of list place `item` (-1 past the list), the
+// tiles without tokens, one each.  The size is the one at which all parts fit one round of
+// workgroups (a few steps from below; a few more than that take as long as a whole round); many
+// query rows of uneven lengths may be better off with two rounds of smaller parts.  In key tiles
+// of a CU: the workgroups that share one take as many times the longest part, all of them at
+// least all tiles over the CUs, and a part costs about nine tiles (its results, written and
+// read, and its start).  6 rows of up to 6000 tokens 173 -> 147 us with two rounds, 512 new
+// tokens at 8192 77 against 95.  Returns the batch row of list place `item` (-1 past the list), the
 // places before it and its parts.  Wave-wide; lanes hold batch rows.
 struct Share {
   int b, before, parts;
@@ -197,6 +204,15 @@ __device__ __forceinline__ int wave_scan(int v) {
   return v;
 }
 __device__ __forceinline__ int wave_sum(int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); }
+__device__ __forceinline__ int wave_max(int v) {  // of values >= 0
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false));
+  v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(v, 63);
+}
 // ceil(n / size) for 1 <= n, size <= 2^17: the quotient of n - 1/2 is never within rounding of a whole
 // number.
 __device__ __forceinline__ int parts_of(int n, float inv_size) {
@@ -217,18 +233,33 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int lane)
     total += t.count * t.n;
   }
   total = wave_sum(total) * p.num_kv_heads;
-  int size = max((total + p.target - 1) / p.target, kMinPart);
-  float inv = 1.f / (float)size;
-  for (int step = 0; step < 4; ++step) {
-    int wgs = t0.count * parts_of(t0.n, inv);
-    for (int i0 = 64; i0 < p.batch; i0 += 64) {
-      const RowTiles t = tiles_of(i0 + lane);
-      wgs += t.count * parts_of(t.n, inv);
+  float inv = 0.f;
+  int64_t best = INT64_MAX;
+  for (int round = 0; round < 2; ++round) {
+    const int target = round ? p.target2 : p.target;
+    if (target == 0) break;
+    int size = max((total + target - 1) / target, kMinPart), wgs = 0, longest = 0;
+    float inv_size = 1.f / (float)size;
+    for (int step = 0; step < 5; ++step) {
+      const int parts = parts_of(t0.n, inv_size);
+      wgs = t0.count * parts;
+      longest = parts_of(t0.n, 1.f / (float)parts);
+      for (int i0 = 64; i0 < p.batch; i0 += 64) {
+        const RowTiles t = tiles_of(i0 + lane);
+        const int more = parts_of(t.n, inv_size);
+        wgs += t.count * more;
+        longest = max(longest, parts_of(t.n, 1.f / (float)more));
+      }
+      wgs = wave_sum(wgs) * p.num_kv_heads;
+      if (wgs <= target || step == 4) break;
+      size = max((int)((float)size * (float)wgs / (float)target), size + 1);
+      inv_size = 1.f / (float)size;
     }
-    wgs = wave_sum(wgs) * p.num_kv_heads;
-    if (wgs <= p.target) break;
-    size = max((int)((float)size * (float)wgs / (float)p.target), size + 1);
-    inv = 1.f / (float)size;
+    const int64_t cost = max((int64_t)((wgs + 255) / 256 * 256) * wave_max(longest), (int64_t)total) + 9 * wgs;
+    if (cost < best) {
+      best = cost;
+      inv = inv_size;
+    }
   }
   Share s = {-1, 0, 1};
   int before = 0;
@@ -692,9 +723,18 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
     if (p.chunk < 0) break;
     const int key0 = k0 + 16 * kT * c + 4 * g;  // lane's key of score e: key0 + 16 (e / 4) + e % 4
     floatx4 s[NB][kT];
+    // -slope |pos - key|; where every key is before its row (!kMasked) the difference is linear
+    float slope[NB], back0[NB];
+    if (kMod & kBias) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) {
+        slope[j] = s_slope[16 * j + col];
+        back0[j] = (float)(s_pos[16 * j + col] - key0) * (kMasked ? 1.f : -slope[j]);
+      }
+    }
     auto bias = [&](int j, int e) {
-      return -s_slope[16 * j + col] *
-             __builtin_fabsf((float)(s_pos[16 * j + col] - key0 - 16 * (e >> 2) - (e & 3)));
+      const float at = (float)(16 * (e >> 2) + (e & 3));
+      return kMasked ? -slope[j] * __builtin_fabsf(back0[j] - at) : __builtin_fmaf(slope[j], at, back0[j]);
     };
 #pragma unroll
     for (int j = 0; j < NB; ++j)
@@ -1003,7 +1043,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
 // are added up through LDS at the end.  Bound by the stream of K and V: with the rows of one
 // wave and shared tiles, 2.9 TB/s.
 template <int NB, int kD, int kMod>
-__global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, kD == 64 ? 4 : 2) void narrow_kernel(Params p) {
   typedef Tile<kD> T;
   constexpr int kRows = 16 * NB;
   __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
@@ -1153,9 +1193,9 @@ __global__ __launch_bounds__(kThreads, kD == 64 && NB < 4 ? 4 : 2) void narrow_k
 
 // Adds the parts of each query row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  Four
 // columns a lane; grid (rows of a batch row, batch).  Batch rows that were not cut, and row tiles
-// without a token, were written by the kernel above.  All loads of kMergeParts parts are issued at once.
+// without a token, were written by the kernel above.  All loads of three or eight parts are issued
+// at once.
 constexpr int kMergeThreads = 256;
-constexpr int kMergeParts = 8;
 template <int kD>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
   constexpr int kLanes = kD / 4;  // of a row
@@ -1185,28 +1225,35 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
     const int64_t step = (int64_t)rt.count * p.num_kv_heads * p.part_rows;
     const int64_t slot0 = ((int64_t)(before + rt.first + rt.count - 1 - tile) * p.num_kv_heads + kvh) *
                               p.part_rows + kr - tile * p.tile_rows;
-    for (int s0 = 0; s0 < used; s0 += kMergeParts) {
-      float ms[kMergeParts], ls[kMergeParts];
-      floatx4 os[kMergeParts];
+    auto add = [&](auto most) {
+      constexpr int kParts = decltype(most)::value;
+      for (int s0 = 0; s0 < used; s0 += kParts) {
+        float ms[kParts], ls[kParts];
+        floatx4 os[kParts];
 #pragma unroll
-      for (int k = 0; k < kMergeParts; ++k) {
-        const int64_t slot = slot0 + min(s0 + k, used - 1) * step;
-        ms[k] = p.part_ml[slot * 2];
-        ls[k] = p.part_ml[slot * 2 + 1];
-        os[k] = *(const floatx4*)(p.part_o + slot * kD + d);
+        for (int k = 0; k < kParts; ++k) {
+          const int64_t slot = slot0 + min(s0 + k, used - 1) * step;
+          ms[k] = p.part_ml[slot * 2];
+          ls[k] = p.part_ml[slot * 2 + 1];
+          os[k] = *(const floatx4*)(p.part_o + slot * kD + d);
+        }
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+          // (a part without a visible key has l = 0; a NaN is not)
+          const bool use = s0 + k < used && __builtin_bit_cast(uint32_t, ls[k]) != 0;
+          const float mn = fmaxf(m, use ? ms[k] : kNegBig);
+          const float a = fast_exp2(m - mn), e = use ? fast_exp2(ms[k] - mn) : 0.f;
+          l = l * a + (use ? ls[k] : 0.f) * e;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[c] = o[c] * a + (use ? os[k][c] : 0.f) * e;
+          m = mn;
+        }
       }
-#pragma unroll
-      for (int k = 0; k < kMergeParts; ++k) {
-        // (a part without a visible key has l = 0; a NaN is not)
-        const bool use = s0 + k < used && __builtin_bit_cast(uint32_t, ls[k]) != 0;
-        const float mn = fmaxf(m, use ? ms[k] : kNegBig);
-        const float a = fast_exp2(m - mn), e = use ? fast_exp2(ms[k] - mn) : 0.f;
-        l = l * a + (use ? ls[k] : 0.f) * e;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[c] = o[c] * a + (use ? os[k][c] : 0.f) * e;
-        m = mn;
-      }
-    }
+    };
+    if (used <= 3)
+      add(std::integral_constant<int, 3>());
+    else
+      add(std::integral_constant<int, 8>());
   }
   const float inv = __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
   if (d < p.head_dim)
@@ -1214,33 +1261,76 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
         to_half4(o * inv);
 }
 
-// How a call is cut: row blocks per wave, row tiles per (batch row, kv head), list entries and
-// results' rows of the parts (0: not cut).
+// How a call is cut: row blocks per wave, row tiles per (batch row, kv head), parts aimed at (0: not
+// cut) and rows of a part's results.
 constexpr int64_t kMaxWgs = (1 << 24) - 1;  // a launch takes fewer than 2^32 threads along x
 struct Plan {
   bool narrow;
   int nb;
-  int64_t row_tiles, wgs, target, part_rows, width;
+  int64_t row_tiles, wgs, target, target2, part_rows, width;
   int64_t tile_rows() const { return narrow ? 16 * nb : 64 * nb; }
+  int64_t parts() const { return std::max(target, target2); }
   size_t bytes(int64_t batch) const {
-    return (size_t)((target + wgs) * part_rows * (width + 2) + 2 * batch) * sizeof(float);
+    return (size_t)((parts() + wgs) * part_rows * (width + 2) + 2 * batch) * sizeof(float);
   }
 };
+
+// Up to 32 rows per kv head: the narrow form, cut into one round of workgroups (two per CU, four
+// of the 64-wide form); with 48 rows it takes four blocks, too many registers, 59 us against 35
+// for 8 x 12 tokens at 4000.  More rows: 1, 2 or 3 row blocks per wave, cut or not, by
+// the estimate that fits what was measured.  A key tile takes a workgroup alone on its CU
+// `alone` us and costs the CU `shared` us where more of them run there: 1.17, 1.74, 2.08 and 0.72,
+// 1.1, 1.5 for 1, 2, 3 blocks (128 wide; chunks of 512 tokens at 8192, 2 x 1000 at 5000, 2 x 2048
+// at 16384).  A call costs 6 us besides, one that is cut 6 more, and a round of parts 6 us per
+// block for results written and read.  Rows of one call that have their own lengths are taken to
+// have two thirds of the bound on average, the longest the whole.  Against three blocks always: 4 x 128
+// tokens at 300 29 -> 14 us, a prompt of 512 25 -> 16, 2 x 1000 at 5000 214 -> 175.
 static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads,
-                 int64_t num_tokens, int64_t head_dim) {
+                 int64_t num_tokens, int64_t head_dim, int64_t window, bool lens,
+                 bool may_cut) {
+  constexpr int64_t kCus = 256;
   const int64_t rows = chunk * (num_q_heads / num_kv_heads);
-  Plan pl;
+  Plan pl = {};
   pl.width = head_dim <= 64 ? 64 : 128;
-  pl.narrow = rows <= 64;
-  const int64_t blocks = (rows + 15) / 16;
-  pl.nb = pl.narrow ? (blocks <= 2 ? (int)blocks : 4) : rows <= 128 ? 2 : 3;
-  const int64_t tile_rows = pl.tile_rows();
-  pl.row_tiles = (rows + tile_rows - 1) / tile_rows;
-  pl.wgs = batch * num_kv_heads * pl.row_tiles;
-  // workgroups resident at once: two per CU, four of the narrow 64-wide form
-  const int64_t slots = pl.narrow && pl.width == 64 && pl.nb < 4 ? 1024 : 512;
-  pl.target = pl.wgs < slots && num_tokens > kMinPart * kKTile ? slots : 0;
-  pl.part_rows = pl.target ? std::min<int64_t>(rows, tile_rows) : 0;
+  pl.narrow = rows <= 32;
+  auto shape = [&](int nb) {
+    pl.nb = nb;
+    pl.row_tiles = (rows + pl.tile_rows() - 1) / pl.tile_rows();
+    pl.wgs = batch * num_kv_heads * pl.row_tiles;
+  };
+  if (pl.narrow) {
+    shape((int)((rows + 15) / 16));
+    const int64_t slots = pl.width == 64 ? 4 * kCus : 2 * kCus;
+    pl.target = may_cut && pl.wgs < slots && num_tokens > kMinPart * kKTile ? slots : 0;
+  } else {
+    static constexpr double kAlone[3] = {1.17, 1.74, 2.08}, kShared[3] = {0.72, 1.1, 1.5};
+    const double wide = pl.width == 64 ? 0.6 : 1.0;
+    const bool ragged = lens && batch > 1;
+    double best = 0;
+    int nb = 0;
+    bool cut = false;
+    for (int i = 1; i <= 3; ++i) {
+      shape(i);
+      const int64_t span = window + pl.tile_rows() / (num_q_heads / num_kv_heads) + kKTile;
+      const double n = (double)((std::min(num_tokens, span) + kKTile - 1) / kKTile);
+      const double alone = wide * kAlone[i - 1], shared = wide * kShared[i - 1];
+      const int64_t per_cu = (pl.wgs + kCus - 1) / kCus;
+      const double whole = 6 + n * (per_cu == 1 ? alone : (double)per_cu * shared);
+      if (nb == 0 || whole < best) best = whole, nb = i, cut = false;
+      const int64_t parts = std::min<int64_t>(2 * kCus / pl.wgs, (int64_t)n / kMinPart);
+      if (may_cut && pl.wgs < 2 * kCus && (parts >= 2 || (ragged && n > 2 * kMinPart))) {
+        const double round = std::min(1.0, (double)(pl.wgs * std::max<int64_t>(parts, 1)) / (2 * kCus));
+        double chain = ceil(n / (double)std::max<int64_t>(parts, 1));
+        if (ragged) chain = (0.65 + 0.7 / (double)batch) * n * (double)pl.wgs / (2 * kCus);
+        const double pieces = 12 + chain * (round <= 0.5 && !ragged ? alone : 2 * shared) + 6 * wide * i * (ragged ? 1.0 : round);
+        if (pieces < best) best = pieces, nb = i, cut = true;
+      }
+    }
+    shape(nb);
+    pl.target = cut ? 2 * kCus : 0;
+    pl.target2 = cut && ragged ? 4 * kCus : 0;
+  }
+  pl.part_rows = pl.target ? std::min<int64_t>(rows, pl.tile_rows()) : 0;
   return pl;
 }
 
@@ -1254,10 +1344,10 @@ static void launch(const Plan& pl, dim3 grid, hipStream_t st, const Params& p) {
   const dim3 block(kThreads);
   if (pl.narrow && pl.nb == 1)
     hipLaunchKernelGGL((narrow_kernel<1, kD, kMod>), grid, block, 0, st, p);
-  else if (pl.narrow && pl.nb == 2)
-    hipLaunchKernelGGL((narrow_kernel<2, kD, kMod>), grid, block, 0, st, p);
   else if (pl.narrow)
-    hipLaunchKernelGGL((narrow_kernel<4, kD, kMod>), grid, block, 0, st, p);
+    hipLaunchKernelGGL((narrow_kernel<2, kD, kMod>), grid, block, 0, st, p);
+  else if (pl.nb == 1)
+    hipLaunchKernelGGL((chunk_kernel<1, kD, kMod>), grid, block, 0, st, p);
   else if (pl.nb == 2)
     hipLaunchKernelGGL((chunk_kernel<2, kD, kMod>), grid, block, 0, st, p);
   else
@@ -1284,8 +1374,14 @@ extern "C" size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t
       max_num_tokens <= 0 || max_num_tokens > kMaxTokens || !fi::head_dim_ok(head_dim) ||
       batch > 0x7fffffff || num_new > 0x7fffffff / num_q_heads)
     return 0;
-  const Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens, head_dim);
-  return pl.target ? pl.bytes(batch) : 0;
+  // whether the call will have lengths of its own, or a window, is not known here: the most of these
+  size_t bytes = 0;
+  for (const bool lens : {false, true}) {
+    const Plan pl =
+        plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens, head_dim, kNoWindow, lens, true);
+    if (pl.target) bytes = std::max(bytes, pl.bytes(batch));
+  }
+  return bytes;
 }
 
 extern "C" int fi_paged_chunk_attention_fwd(
@@ -1390,12 +1486,14 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.window = window == 0 || window > kNoWindow ? kNoWindow : (int)window;
   p.prefix_lens = prefix_lens;
 
-  Plan pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens, head_dim);
+  Plan pl =
+      plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens, head_dim, p.window, context_lens, true);
+  if (pl.target && (!workspace || workspace_bytes < pl.bytes(batch)))
+    pl = plan(batch, num_new, num_q_heads, num_kv_heads, num_tokens, head_dim, p.window, context_lens, false);
   if (pl.wgs > kMaxWgs) {
     set_error("%s: too many new tokens (%lld rows of %lld)", fn, (long long)batch, (long long)num_new);
     return FI_ERR_UNSUPPORTED;
   }
-  if (pl.target && (!workspace || workspace_bytes < pl.bytes(batch))) pl.target = 0;
   p.tile_rows = (int)pl.tile_rows();
   p.tile_div = fast_div((uint32_t)p.tile_rows);
   p.row_tiles = (int)pl.row_tiles;
@@ -1405,13 +1503,14 @@ extern "C" int fi_paged_chunk_attention_fwd(
       return FI_ERR_INVALID;
     }
     p.target = (int)pl.target;
+    p.target2 = (int)pl.target2;
     p.part_rows = (int)pl.part_rows;
     p.part_o = (float*)workspace;
-    p.part_ml = p.part_o + (pl.target + pl.wgs) * pl.part_rows * pl.width;
-    p.shares = (int32_t*)(p.part_ml + (pl.target + pl.wgs) * pl.part_rows * 2);
+    p.part_ml = p.part_o + (pl.parts() + pl.wgs) * pl.part_rows * pl.width;
+    p.shares = (int32_t*)(p.part_ml + (pl.parts() + pl.wgs) * pl.part_rows * 2);
   }
-  // list entries: at most target / num_kv_heads (rounded up) and one per row tile
-  const int64_t items = batch * pl.row_tiles + pl.target / num_kv_heads;
+  // list entries: at most parts() / num_kv_heads and one per row tile
+  const int64_t items = batch * pl.row_tiles + pl.parts() / num_kv_heads;
   const dim3 grid((unsigned)(items * num_kv_heads));
   const hipStream_t st = (hipStream_t)stream;
   const int mod = (softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0);

@@ -92,14 +92,13 @@ def test_chunk_workspace_size(lib):
     for bad in ((0, 4, 24, 8, 4096, 128), (1, 0, 24, 8, 4096, 128), (1, 4, 20, 8, 4096, 128),
                 (1, 4, 24, 8, 0, 128), (1, 4, 24, 8, 4096, 60), (1, 4, 24, 8, (1 << 22) + 1, 128)):
         assert size(*bad) == 0
-    # grows with the bound of the lengths, and is bounded itself
+    # bounded whatever the sizes
     rng = random.Random(3)
     for _ in range(200):
         batch, new = rng.randint(1, 64), rng.randint(1, 600)
         group, hkv = rng.randint(1, 16), rng.randint(1, 16)
         sizes = [size(batch, new, group * hkv, hkv, n, 128) for n in (64, 300, 1000, 5000, 1 << 17, 1 << 22)]
-        assert sizes == sorted(sizes)
-        assert sizes[-1] <= 2048 * min(192, new * group) * 130 * 4 + 8 * batch
+        assert max(sizes) <= 1536 * min(192, new * group) * 130 * 4 + 8 * batch
 
 
 @pytest.mark.parametrize("bad,rc,text", [
