@@ -22,6 +22,7 @@
 //   * Few query rows: the row tile's list of key tiles is cut into parts, by its own true
 //     length, on the device; the parts' unnormalised results are added by a second kernel.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 #include <type_traits>
 
@@ -189,10 +190,15 @@ __device__ __forceinline__ RowTiles row_tiles_of(const Params& p, const Row& row
 // least all tiles over the CUs, and a part costs about nine tiles (its results, written and
 // read, and its start).  6 rows of up to 6000 tokens 173 -> 147 us with two rounds, 512 new
 // tokens at 8192 77 against 95.  Returns the batch row of list place `item` (-1 past the list), the
-// places before it and its parts.  Wave-wide; lanes hold batch rows.
+// places before it and its parts.  For the whole workgroup; s_tiles: an int of LDS per batch row (fewer
+// than 2^10, a call of more workgroups than that is not cut).
 struct Share {
   int b, before, parts;
 };
+// A barrier for LDS: copies stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
 // Inclusive sums over the lanes (row shifts, then row broadcasts: no LDS round trips).
 __device__ __forceinline__ int wave_scan(int v) {
   v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
@@ -218,44 +224,49 @@ __device__ __forceinline__ int wave_max(int v) {  // of values >= 0
 __device__ __forceinline__ int parts_of(int n, float inv_size) {
   return n > 0 ? (int)(((float)n - 0.5f) * inv_size) + 1 : 1;
 }
-__device__ __forceinline__ Share find_share(const Params& p, int item, int lane) {
+__device__ __forceinline__ Share find_share(const Params& p, int item, int tid, int* s_tiles) {
   if (p.batch == 1) {
     const RowTiles t = row_tiles_of(p, row_of(p, 0));
     const int most = max(p.target / max(t.count * p.num_kv_heads, 1), 1);  // parts in one round
     const int parts = max(min(most, (t.n + kMinPart - 1) / kMinPart), 1);
     return {item < t.count * parts + p.row_tiles - t.count ? 0 : -1, 0, parts};
   }
-  auto tiles_of = [&](int i) { return i < p.batch ? row_tiles_of(p, row_of(p, i)) : RowTiles{0, 0, 0}; };
-  const RowTiles t0 = tiles_of(lane);
-  int total = t0.count * t0.n;
-  for (int i0 = 64; i0 < p.batch; i0 += 64) {
-    const RowTiles t = tiles_of(i0 + lane);
-    total += t.count * t.n;
+  // row tiles (fewer than 2^10) and key tiles (at most 2^16 + 1) of every batch row, into LDS
+  constexpr int kShift = 17, kMask = (1 << kShift) - 1;
+  for (int i = tid; i < p.batch; i += kThreads) {
+    const RowTiles t = row_tiles_of(p, row_of(p, i));
+    s_tiles[i] = t.count << kShift | t.n;
+  }
+  lds_barrier();
+  const int lane = tid & 63;
+  int total = 0;
+  for (int i = 0; i < p.batch; i += 64) {
+    const int v = i + lane < p.batch ? s_tiles[i + lane] : 0;
+    total += (v >> kShift) * (v & kMask);
   }
   total = wave_sum(total) * p.num_kv_heads;
   float inv = 0.f;
-  int64_t best = INT64_MAX;
+  int best = INT_MAX;
   for (int round = 0; round < 2; ++round) {
     const int target = round ? p.target2 : p.target;
     if (target == 0) break;
-    int size = max((total + target - 1) / target, kMinPart), wgs = 0, longest = 0;
+    const float inv_target = 1.f / (float)target;
+    int size = max(parts_of(total, inv_target), kMinPart), wgs = 0, longest = 0;
     float inv_size = 1.f / (float)size;
     for (int step = 0; step < 5; ++step) {
-      const int parts = parts_of(t0.n, inv_size);
-      wgs = t0.count * parts;
-      longest = parts_of(t0.n, 1.f / (float)parts);
-      for (int i0 = 64; i0 < p.batch; i0 += 64) {
-        const RowTiles t = tiles_of(i0 + lane);
-        const int more = parts_of(t.n, inv_size);
-        wgs += t.count * more;
-        longest = max(longest, parts_of(t.n, 1.f / (float)more));
+      wgs = longest = 0;
+      for (int i = 0; i < p.batch; i += 64) {
+        const int v = i + lane < p.batch ? s_tiles[i + lane] : 0;
+        const int parts = parts_of(v & kMask, inv_size);
+        wgs += (v >> kShift) * parts;
+        longest = max(longest, parts_of(v & kMask, 1.f / (float)parts));
       }
       wgs = wave_sum(wgs) * p.num_kv_heads;
       if (wgs <= target || step == 4) break;
-      size = max((int)((float)size * (float)wgs / (float)target), size + 1);
+      size = max((int)((float)size * (float)wgs * inv_target), size + 1);
       inv_size = 1.f / (float)size;
     }
-    const int64_t cost = max((int64_t)((wgs + 255) / 256 * 256) * wave_max(longest), (int64_t)total) + 9 * wgs;
+    const int cost = max((wgs + 255) / 256 * 256 * wave_max(longest), total) + 9 * wgs;
     if (cost < best) {
       best = cost;
       inv = inv_size;
@@ -263,20 +274,21 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int lane)
   }
   Share s = {-1, 0, 1};
   int before = 0;
-  for (int i0 = 0; i0 < p.batch; i0 += 64) {
-    const RowTiles t = i0 == 0 ? t0 : tiles_of(i0 + lane);
-    const int parts = parts_of(t.n, inv);
-    const int items = i0 + lane < p.batch ? t.count * parts + p.row_tiles - t.count : 0;
+  for (int i = 0; i < p.batch; i += 64) {
+    const int v = i + lane < p.batch ? s_tiles[i + lane] : 0;
+    const int parts = parts_of(v & kMask, inv);
+    const int items = i + lane < p.batch ? (v >> kShift) * (parts - 1) + p.row_tiles : 0;
     const int upto = before + wave_scan(items);
     if (const uint64_t hit = __builtin_amdgcn_ballot_w64(upto > item)) {
       const int l = __builtin_ctzll(hit);
-      s.b = i0 + l;
+      s.b = i + l;
       s.before = __builtin_amdgcn_readlane(upto - items, l);
       s.parts = __builtin_amdgcn_readlane(parts, l);
-      return s;
+      break;
     }
     before = __builtin_amdgcn_readlane(upto, 63);
   }
+  lds_barrier();  // the tiles that follow take this place
   return s;
 }
 
@@ -355,10 +367,6 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
-// The same for LDS only: copies stay on their way.
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
 // 16 bits of each wave, as one scalar.
 __device__ __forceinline__ uint64_t uniform64(const uint16_t* x) {
   const uint64_t v = *(const uint64_t*)x;
@@ -857,13 +865,13 @@ struct Job {
   Row row;
   Span span;
 };
-__device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows, Job& job) {
+__device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows, int* s_tiles, Job& job) {
   job.kvh = blockIdx.x % p.num_kv_heads;
   const int item = blockIdx.x / p.num_kv_heads;
   int tile, part = 0;
   job.parts = 1;
   if (p.part_o) {
-    const Share s = find_share(p, item, tid & 63);
+    const Share s = find_share(p, item, tid, s_tiles);
     if (s.b < 0) return false;  // past the list
     job.b = s.b;
     const RowTiles rt = row_tiles_of(p, row_of(p, job.b));
@@ -913,7 +921,7 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   const int col = lane & 15;
   const int g = lane >> 4;
   Job job;
-  if (!find_job(p, tid, kRows, job)) return;
+  if (!find_job(p, tid, kRows, (int*)stages, job)) return;
   const int b = job.b, kvh = job.kvh, r0 = job.r0, first = job.first, n = job.n;
   const Row& row = job.row;
   const Span& span = job.span;
@@ -1061,7 +1069,7 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 4 : 2) void narrow_kernel(Para
   const int col = lane & 15;
   const int g = lane >> 4;
   Job job;
-  if (!find_job(p, tid, kRows, job)) return;
+  if (!find_job(p, tid, kRows, (int*)stages, job)) return;
   const int b = job.b, kvh = job.kvh, r0 = job.r0, first = job.first, n = job.n;
   const Row& row = job.row;
   const Span& span = job.span;

@@ -221,33 +221,37 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
     one row stride) and returned as that tensor."""
     _need_cuda("x", x)
     _need_cuda("residual", residual)
-    hidden = x.shape[-1]
-    if residual.shape != x.shape:
-        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(x.shape)}")
-    if residual.get_device() != x.get_device():
+    shape = x.shape
+    if residual.shape != shape:
+        raise ValueError(f"residual {tuple(residual.shape)} does not match x {tuple(shape)}")
+    dev = x.get_device()
+    if residual.get_device() != dev:
         raise RuntimeError("residual must be on the same device as x")
     if x.dtype is not torch.float16 or residual.dtype is not torch.float16:
         raise TypeError(f"x and residual must be float16, got {x.dtype} / {residual.dtype}")
+    hidden = shape[-1]
     if weight.shape != (hidden,):
         raise ValueError(f"weight {tuple(weight.shape)} does not match hidden {hidden}")
-    wt = _norm_weight(weight, x)
-    x2, x_stride, x_ptr = _rows16(x.reshape(-1, hidden), 2)
-    r2, r_stride, r_ptr = _rows16(residual.reshape(-1, hidden), 2)
+    if weight.dtype is not torch.float16 or weight.get_device() != dev or not weight.is_contiguous():
+        weight = _norm_weight(weight, x)
+    flat = len(shape) == 2
+    x2, x_stride, x_ptr = _rows16(x if flat else x.reshape(-1, hidden), 2)
+    r2, r_stride, r_ptr = _rows16(residual if flat else residual.reshape(-1, hidden), 2)
     rows = x2.shape[0]
-    out = torch.empty(rows, hidden, dtype=torch.float16, device=x.device)
+    out = torch.empty_like(x, memory_format=torch.contiguous_format)
     if inplace:
         if rows and r_ptr != residual.data_ptr():
             raise ValueError("an in-place residual needs 16-byte aligned rows at one row stride")
         h, h_stride, h_ptr = residual, r_stride, r_ptr
     else:
-        h = torch.empty(x.shape, dtype=torch.float16, device=x.device)
+        h = torch.empty_like(x, memory_format=torch.contiguous_format)
         h_stride, h_ptr = hidden, h.data_ptr()
     if rows:
         rc = _lib.calls().fi_add_rmsnorm(x_ptr, x_stride, r_ptr, r_stride, rows, hidden,
-                                        wt.data_ptr(), float(eps), h_ptr, h_stride, out.data_ptr(),
+                                        weight.data_ptr(), float(eps), h_ptr, h_stride, out.data_ptr(),
                                         hidden, _lib.tensor_stream(x))
         _lib.check(rc, "add_rms_norm")
-    return out.reshape(x.shape), h
+    return out, h
 
 
 def rms_norm_int4_matmul(x: torch.Tensor, norm_weight: torch.Tensor, w, eps: float = 1e-5,
