@@ -38,6 +38,9 @@ constexpr float kLazyLog2 = 8.f;  // the reference max may lag the true max by 2
 constexpr int kNoWindow = 0x3fffffff;
 constexpr int64_t kMaxTokens = (int64_t)1 << 22;
 constexpr int kMinPart = 2;  // key tiles of the smallest part
+// Calls of few query rows and up to this many tokens are not cut: adding the parts takes as long as
+// the key tiles they save (one token of 256 11.8 against 8.6 us).
+constexpr int64_t kWholeTokens = 512;
 // Largest cap whose tanh is taken from exp2 alone: its absolute error, about 2e-7, times the
 // cap is an error of the logit, here 1e-4.
 constexpr float kExpCap = 500.f;
@@ -1201,16 +1204,33 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 4 : 2) void narrow_kernel(Para
 
 // Adds the parts of each query row: o = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s.  Four
 // columns a lane; grid (rows of a batch row, batch).  Batch rows that were not cut, and row tiles
-// without a token, were written by the kernel above.  All loads of three or eight parts are issued
-// at once.
+// without a token, were written by the kernels above.  All loads of a few parts are issued at once;
+// with kSpread (few rows in many parts) the workgroup has one row and each kD / 4 lanes every
+// 1024 / kD-th part, added up through LDS.
 constexpr int kMergeThreads = 256;
-template <int kD>
+struct Sum {
+  float m = kNegBig, l = 0.f;
+  floatx4 o = {0.f, 0.f, 0.f, 0.f};
+  // (a part without a visible key has l = 0; a NaN is not)
+  __device__ __forceinline__ void add(bool use, float ms, float ls, floatx4 os) {
+    use = use && __builtin_bit_cast(uint32_t, ls) != 0;
+    const float mn = fmaxf(m, use ? ms : kNegBig);
+    const float a = fast_exp2(m - mn), e = use ? fast_exp2(ms - mn) : 0.f;
+    l = l * a + (use ? ls : 0.f) * e;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = o[c] * a + (use ? os[c] : 0.f) * e;
+    m = mn;
+  }
+};
+template <int kD, bool kSpread>
 __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
   constexpr int kLanes = kD / 4;  // of a row
+  constexpr int kGroups = kMergeThreads / kLanes;
   const int b = blockIdx.y;
   const int before = p.shares[2 * b], parts = p.shares[2 * b + 1];
   if (parts <= 1) return;
-  const int r = blockIdx.x * (kMergeThreads / kLanes) + threadIdx.x / kLanes;  // (token, query head)
+  const int group = threadIdx.x / kLanes;
+  const int r = kSpread ? blockIdx.x : blockIdx.x * kGroups + group;  // (token, query head)
   const int d = 4 * (threadIdx.x % kLanes);
   if (r >= p.chunk * p.num_q_heads) return;
   const int t = r / p.num_q_heads;
@@ -1222,8 +1242,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
   const int kr = t * p.group + h - kvh * p.group;
   const int tile = div_by(kr, p.tile_div);
   if (tile < rt.first || tile >= rt.first + rt.count) return;
-  floatx4 o = {0.f, 0.f, 0.f, 0.f};
-  float m = kNegBig, l = 0.f;
+  Sum sum;
   if (pos >= 0 && pos < row.len) {
     int lo, hi;
     row_positions(p, row, tile * p.tile_rows, (tile + 1) * p.tile_rows - 1, lo, hi);
@@ -1234,39 +1253,45 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
     const int64_t slot0 = ((int64_t)(before + rt.first + rt.count - 1 - tile) * p.num_kv_heads + kvh) *
                               p.part_rows + kr - tile * p.tile_rows;
     auto add = [&](auto most) {
-      constexpr int kParts = decltype(most)::value;
-      for (int s0 = 0; s0 < used; s0 += kParts) {
+      constexpr int kParts = decltype(most)::value, kStep = kSpread ? kGroups : 1;
+      for (int s0 = kSpread ? group : 0; s0 < used; s0 += kParts * kStep) {
         float ms[kParts], ls[kParts];
         floatx4 os[kParts];
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
-          const int64_t slot = slot0 + min(s0 + k, used - 1) * step;
+          const int64_t slot = slot0 + min(s0 + k * kStep, used - 1) * step;
           ms[k] = p.part_ml[slot * 2];
           ls[k] = p.part_ml[slot * 2 + 1];
           os[k] = *(const floatx4*)(p.part_o + slot * kD + d);
         }
 #pragma unroll
-        for (int k = 0; k < kParts; ++k) {
-          // (a part without a visible key has l = 0; a NaN is not)
-          const bool use = s0 + k < used && __builtin_bit_cast(uint32_t, ls[k]) != 0;
-          const float mn = fmaxf(m, use ? ms[k] : kNegBig);
-          const float a = fast_exp2(m - mn), e = use ? fast_exp2(ms[k] - mn) : 0.f;
-          l = l * a + (use ? ls[k] : 0.f) * e;
-#pragma unroll
-          for (int c = 0; c < 4; ++c) o[c] = o[c] * a + (use ? os[k][c] : 0.f) * e;
-          m = mn;
-        }
+        for (int k = 0; k < kParts; ++k) sum.add(s0 + k * kStep < used, ms[k], ls[k], os[k]);
       }
     };
-    if (used <= 3)
+    if (used <= 3 * (kSpread ? kGroups : 1))
       add(std::integral_constant<int, 3>());
     else
       add(std::integral_constant<int, 8>());
   }
-  const float inv = __builtin_bit_cast(uint32_t, l) != 0 ? 1.f / l : 0.f;
+  if constexpr (kSpread) {  // the row's groups, in order
+    __shared__ floatx4 s_o[kMergeThreads];
+    __shared__ float s_m[kMergeThreads], s_l[kMergeThreads];
+    s_o[threadIdx.x] = sum.o;
+    s_m[threadIdx.x] = sum.m;
+    s_l[threadIdx.x] = sum.l;
+    __syncthreads();
+    if (group > 0) return;
+    sum = Sum();
+#pragma unroll
+    for (int k = 0; k < kGroups; ++k) {
+      const int x = k * kLanes + threadIdx.x;
+      sum.add(true, s_m[x], s_l[x], s_o[x]);
+    }
+  }
+  const float inv = __builtin_bit_cast(uint32_t, sum.l) != 0 ? 1.f / sum.l : 0.f;
   if (d < p.head_dim)
     *(half4*)(p.o + (int64_t)b * p.o_sb + (int64_t)t * p.o_st + (int64_t)h * p.o_sh + d) =
-        to_half4(o * inv);
+        to_half4(sum.o * inv);
 }
 
 // How a call is cut: row blocks per wave, row tiles per (batch row, kv head), parts aimed at (0: not
@@ -1309,7 +1334,7 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
   if (pl.narrow) {
     shape((int)((rows + 15) / 16));
     const int64_t slots = pl.width == 64 ? 4 * kCus : 2 * kCus;
-    pl.target = may_cut && pl.wgs < slots && num_tokens > kMinPart * kKTile ? slots : 0;
+    pl.target = may_cut && pl.wgs < slots && num_tokens > kWholeTokens ? slots : 0;
   } else {
     static constexpr double kAlone[3] = {1.17, 1.74, 2.08}, kShared[3] = {0.72, 1.1, 1.5};
     const double wide = pl.width == 64 ? 0.6 : 1.0;
@@ -1517,8 +1542,11 @@ extern "C" int fi_paged_chunk_attention_fwd(
     p.part_ml = p.part_o + (pl.parts() + pl.wgs) * pl.part_rows * pl.width;
     p.shares = (int32_t*)(p.part_ml + (pl.parts() + pl.wgs) * pl.part_rows * 2);
   }
-  // list entries: at most parts() / num_kv_heads and one per row tile
-  const int64_t items = batch * pl.row_tiles + pl.parts() / num_kv_heads;
+  // list entries: at most parts() / num_kv_heads and one per row tile, nor more than the smallest
+  // parts of the longest list
+  const int64_t most = (num_tokens + kKTile * kMinPart - 1) / (kKTile * kMinPart);
+  int64_t items = batch * pl.row_tiles;
+  if (pl.target) items = std::min(items + pl.parts() / num_kv_heads, items * std::max<int64_t>(most, 1));
   const dim3 grid((unsigned)(items * num_kv_heads));
   const hipStream_t st = (hipStream_t)stream;
   const int mod = (softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0);
@@ -1528,11 +1556,18 @@ extern "C" int fi_paged_chunk_attention_fwd(
     launch<128>(mod, pl, grid, st, p);
   const int rc = check_launch(fn);
   if (rc != FI_OK || !pl.target) return rc;
-  const int64_t merge_rows = kMergeThreads / (pl.width / 4);
+  // a workgroup per row where the parts per row are many (4 drafted tokens at 1024: eight)
+  const bool spread = pl.target >= 4 * pl.wgs && pl.narrow;
+  const int64_t merge_rows = spread ? 1 : kMergeThreads / (pl.width / 4);
   const dim3 mgrid((unsigned)((num_new * num_q_heads + merge_rows - 1) / merge_rows), (unsigned)batch);
-  if (pl.width == 64)
-    hipLaunchKernelGGL(merge_kernel<64>, mgrid, dim3(kMergeThreads), 0, st, p);
+  const dim3 mblock(kMergeThreads);
+  if (pl.width == 64 && spread)
+    hipLaunchKernelGGL((merge_kernel<64, true>), mgrid, mblock, 0, st, p);
+  else if (pl.width == 64)
+    hipLaunchKernelGGL((merge_kernel<64, false>), mgrid, mblock, 0, st, p);
+  else if (spread)
+    hipLaunchKernelGGL((merge_kernel<128, true>), mgrid, mblock, 0, st, p);
   else
-    hipLaunchKernelGGL(merge_kernel<128>, mgrid, dim3(kMergeThreads), 0, st, p);
+    hipLaunchKernelGGL((merge_kernel<128, false>), mgrid, mblock, 0, st, p);
   return check_launch(fn);
 }

@@ -86,7 +86,7 @@ def test_chunk_empty_calls(lib):
 
 def test_chunk_workspace_size(lib):
     size = lib.fi_paged_chunk_attention_workspace_size
-    assert size(1, 4, 24, 8, 128, 128) == 0         # two tiles of keys: nothing to cut
+    assert size(1, 4, 24, 8, 512, 128) == 0         # a few tiles of keys: not cut
     assert size(64, 512, 24, 8, 4096, 128) == 0     # query tiles alone fill the device
     assert size(1, 4, 24, 8, 4096, 128) > 0
     for bad in ((0, 4, 24, 8, 4096, 128), (1, 0, 24, 8, 4096, 128), (1, 4, 20, 8, 4096, 128),
