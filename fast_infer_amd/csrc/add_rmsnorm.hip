@@ -18,6 +18,12 @@ constexpr int kWaves = 4;
 constexpr int kThreads = kWaves * 64;
 constexpr int kMaxParts = 4;                       // 16-byte pieces a thread holds
 constexpr int kMaxHeld = kThreads * 8 * kMaxParts;  // 8192
+// Rows up to this wide by a wave each, wider ones by a workgroup: 60000 x 256 56 -> 22 us, 16384 x 768
+// 20 -> 18, 30000 x 1024 40 -> 38.
+constexpr int kNarrow = 1024;
+// Bytes moved from which the non-temporal policy pays, beyond the last-level cache: 16384 x 5120
+// 116 -> 110 us (6.1 TB/s); 30000 x 1024 (246 MB) 40 against 42.
+constexpr int64_t kCached = (int64_t)400 << 20;
 
 struct Params {
   const half_t* x;
@@ -67,16 +73,21 @@ __device__ __forceinline__ u32x4 scale8(u32x4 hv, float r, u32x4 wv) {
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_rsrc(const half_t* row, int hidden) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)row, (short)0, hidden * 2, 0x00020000);
 }
+// kNt: the non-temporal policy (2), for calls beyond the last-level cache.
+template <bool kNt>
 __device__ __forceinline__ u32x4 load16(__amdgpu_buffer_rsrc_t r, int byte) {
-  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, 0));
+  return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, byte, 0, kNt ? 2 : 0));
 }
+template <bool kNt>
 __device__ __forceinline__ void store16(__amdgpu_buffer_rsrc_t r, int byte, u32x4 v) {
-  __builtin_amdgcn_raw_buffer_store_b128(v, r, byte, 0, 0);
+  __builtin_amdgcn_raw_buffer_store_b128(v, r, byte, 0, kNt ? 2 : 0);
 }
 
-// A row by kRowWaves waves, kParts pieces a thread.
-template <int kRowWaves, int kParts>
+// A row by kRowWaves waves (1 or all), kParts pieces a thread.  (Workgroups that loop over rows and
+// load the next one ahead were slower: 16384 x 5120 117 to 122 us against 110.)
+template <int kRowWaves, int kParts, bool kNt>
 __global__ __launch_bounds__(kThreads) void held_kernel(Params p) {
+  static_assert(kRowWaves == 1 || kRowWaves == kWaves, "a workgroup's waves share a row, or none do");
   __shared__ float part[kWaves];
   const int lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -90,22 +101,21 @@ __global__ __launch_bounds__(kThreads) void held_kernel(Params p) {
   u32x4 v[kParts], a[kParts], wv[kParts];
 #pragma unroll
   for (int i = 0; i < kParts; ++i) {
-    v[i] = load16(xr, at + i * kStep);
-    a[i] = load16(rr, at + i * kStep);
+    v[i] = load16<kNt>(xr, at + i * kStep);
+    a[i] = load16<kNt>(rr, at + i * kStep);
   }
 #pragma unroll
-  for (int i = 0; i < kParts; ++i) wv[i] = load16(wr, at + i * kStep);
+  for (int i = 0; i < kParts; ++i) wv[i] = load16<false>(wr, at + i * kStep);
   const __amdgpu_buffer_rsrc_t hr = row_rsrc(p.h + row * p.h_stride, p.hidden);
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < kParts; ++i) {
     v[i] = add8(v[i], a[i]);
-    store16(hr, at + i * kStep, v[i]);
+    store16<kNt>(hr, at + i * kStep, v[i]);
     s += sum_sq8(v[i]);
   }
   s = wave_sum(s);
   if (kRowWaves > 1) {
-    static_assert(kRowWaves == 1 || kRowWaves == kWaves, "a workgroup's waves share a row, or none do");
     if (lane == 0) part[w] = s;
     __syncthreads();
     s = part[0] + part[1] + part[2] + part[3];
@@ -113,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void held_kernel(Params p) {
   const float r = rsqrtf(s / (float)p.hidden + p.eps);
   const __amdgpu_buffer_rsrc_t orr = row_rsrc(p.out + row * p.out_stride, p.hidden);
 #pragma unroll
-  for (int i = 0; i < kParts; ++i) store16(orr, at + i * kStep, scale8(v[i], r, wv[i]));
+  for (int i = 0; i < kParts; ++i) store16<kNt>(orr, at + i * kStep, scale8(v[i], r, wv[i]));
 }
 
 // Rows of any length: h is read back (by the thread that wrote it).
@@ -174,16 +184,31 @@ extern "C" int fi_add_rmsnorm(const void* x, int64_t x_stride, const void* resid
   const Params p = {(const half_t*)x, (const half_t*)residual, (const half_t*)weight, (half_t*)h_out,
                     (half_t*)out, x_stride, res_stride, h_stride, out_stride, M, (int)hidden, eps};
   const hipStream_t st = (hipStream_t)stream;
-  const dim3 block(kThreads), grid((unsigned)M);
+  const dim3 block(kThreads);
   if (hidden > kMaxHeld) {
-    hipLaunchKernelGGL(long_kernel, grid, block, 0, st, p);
-  } else {
-    switch ((hidden + kThreads * 8 - 1) / (kThreads * 8)) {
-      case 1: hipLaunchKernelGGL((held_kernel<4, 1>), grid, block, 0, st, p); break;
-      case 2: hipLaunchKernelGGL((held_kernel<4, 2>), grid, block, 0, st, p); break;
-      case 3: hipLaunchKernelGGL((held_kernel<4, 3>), grid, block, 0, st, p); break;
-      default: hipLaunchKernelGGL((held_kernel<4, 4>), grid, block, 0, st, p); break;
-    }
+    hipLaunchKernelGGL(long_kernel, dim3((unsigned)M), block, 0, st, p);
+    return check_launch(fn);
   }
+  const bool nt = M * hidden * 8 > kCached;
+  const bool narrow = hidden <= kNarrow;
+  const int64_t wgs = narrow ? (M + kWaves - 1) / kWaves : M;
+  const dim3 grid((unsigned)wgs);
+  const int parts = (int)((hidden + (narrow ? 512 : 2048) - 1) / (narrow ? 512 : 2048));
+#define FI_ADDNORM(R, P)                                                              \
+  do {                                                                                \
+    if (nt)                                                                           \
+      hipLaunchKernelGGL((held_kernel<R, P, true>), grid, block, 0, st, p);           \
+    else                                                                              \
+      hipLaunchKernelGGL((held_kernel<R, P, false>), grid, block, 0, st, p);          \
+  } while (0)
+  switch (narrow ? -parts : parts) {
+    case -1: FI_ADDNORM(1, 1); break;
+    case -2: FI_ADDNORM(1, 2); break;
+    case 1: FI_ADDNORM(4, 1); break;
+    case 2: FI_ADDNORM(4, 2); break;
+    case 3: FI_ADDNORM(4, 3); break;
+    default: FI_ADDNORM(4, 4); break;
+  }
+#undef FI_ADDNORM
   return check_launch(fn);
 }
