@@ -72,6 +72,7 @@ struct Params {
   int whole;  // block_size % 16 == 0: the 16 keys that a wave copies lie in one block
   FastDiv block_div;
   int num_kv_heads;
+  FastDiv kv_div;
   int64_t row_bytes;  // one pool slot, all kv heads
   const int32_t* block_table;
   int64_t bt_stride;
@@ -82,7 +83,9 @@ struct Params {
   half_t* o;
   int64_t o_sb, o_st, o_sh;
   int batch, chunk;
+  FastDiv batch_div;
   int num_q_heads;
+  FastDiv head_div;
   int group;
   FastDiv group_div;
   int head_dim;
@@ -222,15 +225,19 @@ __device__ __forceinline__ int wave_max(int v) {  // of values >= 0
   v = max(v, __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false));
   return __builtin_amdgcn_readlane(v, 63);
 }
-// ceil(n / size) for 1 <= n, size <= 2^17: the quotient of n - 1/2 is never within rounding of a whole
-// number.
+// ceil(n / size) for n, size <= 2^17 (1 for n = 0), from 1 / size to the last bit or two: n - 1/2 over
+// size is further from a whole number than any rounding here.  Larger n: within one part in 2^22.
+__device__ __forceinline__ float inverse(int x) { return __builtin_amdgcn_rcpf((float)x); }
 __device__ __forceinline__ int parts_of(int n, float inv_size) {
   return n > 0 ? (int)(((float)n - 0.5f) * inv_size) + 1 : 1;
 }
+// floor(n / d) in the same range
+__device__ __forceinline__ int whole_of(int n, int d) { return (int)(((float)n + 0.5f) * inverse(d)); }
+
 __device__ __forceinline__ Share find_share(const Params& p, int item, int tid, int* s_tiles) {
   if (p.batch == 1) {
     const RowTiles t = row_tiles_of(p, row_of(p, 0));
-    const int most = max(p.target / max(t.count * p.num_kv_heads, 1), 1);  // parts in one round
+    const int most = whole_of(p.target, max(t.count * p.num_kv_heads, 1));  // parts in one round
     const int parts = max(min(most, (t.n + kMinPart - 1) / kMinPart), 1);
     return {item < t.count * parts + p.row_tiles - t.count ? 0 : -1, 0, parts};
   }
@@ -242,32 +249,45 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int tid, 
   }
   lds_barrier();
   const int lane = tid & 63;
-  int total = 0;
-  for (int i = 0; i < p.batch; i += 64) {
-    const int v = i + lane < p.batch ? s_tiles[i + lane] : 0;
+  auto tiles_at = [&](int i) { return i + lane < p.batch ? s_tiles[i + lane] : 0; };
+  const int v0 = tiles_at(0);
+  int total = (v0 >> kShift) * (v0 & kMask), rows = v0 >> kShift;
+  for (int i = 64; i < p.batch; i += 64) {
+    const int v = tiles_at(i);
     total += (v >> kShift) * (v & kMask);
+    rows += v >> kShift;
   }
   total = wave_sum(total) * p.num_kv_heads;
+  rows = wave_sum(rows) * p.num_kv_heads;
   float inv = 0.f;
   int best = INT_MAX;
   for (int round = 0; round < 2; ++round) {
     const int target = round ? p.target2 : p.target;
     if (target == 0) break;
-    const float inv_target = 1.f / (float)target;
-    int size = max(parts_of(total, inv_target), kMinPart), wgs = 0, longest = 0;
-    float inv_size = 1.f / (float)size;
+    // no smaller than all tiles over the target (the list's bound); each row tile's last part is
+    // half full on average
+    const int least = max(parts_of(total, inverse(target)), kMinPart);
+    int size = max(parts_of(total, inverse(max(target - rows / 2, 1))), least), wgs = 0, longest = 0;
+    if (2 * rows > target) size = least;
+    float inv_size = inverse(size);
     for (int step = 0; step < 5; ++step) {
-      wgs = longest = 0;
-      for (int i = 0; i < p.batch; i += 64) {
-        const int v = i + lane < p.batch ? s_tiles[i + lane] : 0;
+      const int parts0 = parts_of(v0 & kMask, inv_size);
+      wgs = (v0 >> kShift) * parts0;
+      longest = parts_of(v0 & kMask, inverse(parts0));
+      for (int i = 64; i < p.batch; i += 64) {
+        const int v = tiles_at(i);
         const int parts = parts_of(v & kMask, inv_size);
         wgs += (v >> kShift) * parts;
-        longest = max(longest, parts_of(v & kMask, 1.f / (float)parts));
+        longest = max(longest, parts_of(v & kMask, inverse(parts)));
       }
       wgs = wave_sum(wgs) * p.num_kv_heads;
       if (wgs <= target || step == 4) break;
-      size = max((int)((float)size * (float)wgs * inv_target), size + 1);
-      inv_size = 1.f / (float)size;
+      size = max((int)((float)size * (float)wgs * inverse(target)), size + 1);
+      inv_size = inverse(size);
+    }
+    if (p.target2 == 0) {
+      inv = inv_size;
+      break;
     }
     const int cost = max((wgs + 255) / 256 * 256 * wave_max(longest), total) + 9 * wgs;
     if (cost < best) {
@@ -278,7 +298,7 @@ __device__ __forceinline__ Share find_share(const Params& p, int item, int tid, 
   Share s = {-1, 0, 1};
   int before = 0;
   for (int i = 0; i < p.batch; i += 64) {
-    const int v = i + lane < p.batch ? s_tiles[i + lane] : 0;
+    const int v = i == 0 ? v0 : tiles_at(i);
     const int parts = parts_of(v & kMask, inv);
     const int items = i + lane < p.batch ? (v >> kShift) * (parts - 1) + p.row_tiles : 0;
     const int upto = before + wave_scan(items);
@@ -869,8 +889,8 @@ struct Job {
   Span span;
 };
 __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows, int* s_tiles, Job& job) {
-  job.kvh = blockIdx.x % p.num_kv_heads;
-  const int item = blockIdx.x / p.num_kv_heads;
+  const int item = div_by(blockIdx.x, p.kv_div);
+  job.kvh = blockIdx.x - item * p.num_kv_heads;
   int tile, part = 0;
   job.parts = 1;
   if (p.part_o) {
@@ -881,7 +901,7 @@ __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows
     int at = item - s.before;
     if (at == 0 && job.kvh == 0 && tid < 2) p.shares[2 * job.b + tid] = tid ? s.parts : s.before;
     if (at < rt.count * s.parts) {
-      part = at / rt.count;
+      part = __builtin_amdgcn_readfirstlane(whole_of(at, rt.count));
       job.parts = s.parts;
       tile = rt.first + rt.count - 1 - (at - part * rt.count);
     } else {  // a row tile without tokens
@@ -889,15 +909,18 @@ __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows
       tile = at < rt.first ? at : at + rt.count;
     }
   } else {  // the last row tiles see the most keys: first
-    job.b = item % p.batch;
-    tile = p.row_tiles - 1 - item / p.batch;
+    const int back = div_by(item, p.batch_div);
+    job.b = item - back * p.batch;
+    tile = p.row_tiles - 1 - back;
   }
   job.r0 = tile * tile_rows;
   job.row = row_of(p, job.b);
   int lo, hi;
   row_positions(p, job.row, job.r0, job.r0 + tile_rows - 1, lo, hi);
   job.span = span_of(p, job.row, lo, hi);
-  const int size = (job.span.n + job.parts - 1) / job.parts;
+  const int size =
+      job.parts == 1 ? job.span.n
+                     : __builtin_amdgcn_readfirstlane(parts_of(job.span.n, inverse(job.parts)));
   job.first = min(part * size, job.span.n);
   job.n = min(size, job.span.n - job.first);
   // a short list in few pieces: the other kernel reads no more
@@ -1233,7 +1256,7 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
   const int r = kSpread ? blockIdx.x : blockIdx.x * kGroups + group;  // (token, query head)
   const int d = 4 * (threadIdx.x % kLanes);
   if (r >= p.chunk * p.num_q_heads) return;
-  const int t = r / p.num_q_heads;
+  const int t = div_by(r, p.head_div);
   const int h = r - t * p.num_q_heads;
   const Row row = row_of(p, b);
   const int pos = row.start + t;
@@ -1247,8 +1270,8 @@ __global__ __launch_bounds__(kMergeThreads) void merge_kernel(Params p) {
     int lo, hi;
     row_positions(p, row, tile * p.tile_rows, (tile + 1) * p.tile_rows - 1, lo, hi);
     const int n = span_of(p, row, lo, hi).n;
-    const int size = (n + parts - 1) / parts;
-    const int used = (n + size - 1) / size;  // parts with key tiles
+    const int size = parts_of(n, inverse(parts));
+    const int used = parts_of(n, inverse(size));  // parts with key tiles
     const int64_t step = (int64_t)rt.count * p.num_kv_heads * p.part_rows;
     const int64_t slot0 = ((int64_t)(before + rt.first + rt.count - 1 - tile) * p.num_kv_heads + kvh) *
                               p.part_rows + kr - tile * p.tile_rows;
@@ -1484,6 +1507,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.whole = block_size % 16 == 0;
   p.block_div = fast_div((uint32_t)block_size);
   p.num_kv_heads = (int)num_kv_heads;
+  p.kv_div = fast_div((uint32_t)num_kv_heads);
   p.row_bytes = num_kv_heads * head_dim * 2;
   p.block_table = block_table;
   p.bt_stride = bt_stride;
@@ -1495,8 +1519,10 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.o = (half_t*)o;
   p.o_sb = o_sb; p.o_st = o_st; p.o_sh = o_sh;
   p.batch = (int)batch;
+  p.batch_div = fast_div((uint32_t)batch);
   p.chunk = (int)num_new;
   p.num_q_heads = (int)num_q_heads;
+  p.head_div = fast_div((uint32_t)num_q_heads);
   p.group = (int)(num_q_heads / num_kv_heads);
   p.group_div = fast_div((uint32_t)p.group);
   p.head_dim = (int)head_dim;
