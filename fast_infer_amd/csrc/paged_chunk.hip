@@ -90,13 +90,12 @@ struct Params {
   FastDiv group_div;
   int head_dim;
   int d_chunks;       // 16-byte chunks of a row; those past it are read as zeros
-  float scale_log2;   // score unit -> log2 unit (1 with a cap: those scores are made in log2 units)
+  float scale_log2;   // score unit -> log2 unit
   float lazy_raw;     // kLazyLog2 in score units
   float lazy_log2;    // lazy_raw * scale_log2
   uint32_t q_sign;    // 0x80008000: Q negated (negative sm_scale without a cap)
   int q_zero;         // sm_scale == 0 without a cap: Q read as zeros
   float cap_exp;      // sm_scale / cap * 2 log2(e)
-  float cap_log2;     // cap * log2(e)
   const float* slopes;
   float slope_mul;    // slope unit -> score unit
   int window;
@@ -341,13 +340,20 @@ __device__ __attribute__((aligned(256))) const char g_zeros[2 * kHeadDim] = {0};
 // The table entry of keys that are not to be read.
 __device__ const int32_t g_no_block = -1;
 
+// Values that are the same in every lane, where the compiler has them in vector registers.
+__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ uint32_t scalar(uint32_t x) { return (uint32_t)scalar((int)x); }
+__device__ __forceinline__ uint64_t scalar(uint64_t x) {
+  return (uint64_t)scalar((uint32_t)(x >> 32)) << 32 | scalar((uint32_t)x);
+}
+
 // One direct-to-LDS copy from a 64-bit address per lane: 16 bytes to LDS byte lds + 16 * lane.
 // Through inline asm for the reasons given at lds_copy16; the callers wait for the copies
 // themselves.  M0 takes one idle slot before a global load reads it.
 __device__ __forceinline__ void lds_copy16_global(const char* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
-               : "s"(lds), "v"(src)
+               : "s"(scalar(lds)), "v"(src)
                : "memory");
 }
 
@@ -355,7 +361,7 @@ __device__ __forceinline__ void lds_copy16_global(const char* src, uint32_t lds)
 __device__ __forceinline__ void lds_copy16_global_nt(const char* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt"
                :
-               : "s"(lds), "v"(src)
+               : "s"(scalar(lds)), "v"(src)
                : "memory");
 }
 // The same from a common base and 32-bit offsets.
@@ -364,19 +370,19 @@ __device__ __forceinline__ void lds_copy16_base(const char* base, uint32_t offse
   if (kOnce)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt"
                  :
-                 : "s"(lds), "v"(offset), "s"(base)
+                 : "s"(scalar(lds)), "v"(offset), "s"(scalar((uint64_t)base))
                  : "memory");
   else
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                  :
-                 : "s"(lds), "v"(offset), "s"(base)
+                 : "s"(scalar(lds)), "v"(offset), "s"(scalar((uint64_t)base))
                  : "memory");
 }
 // The same with 4 bytes a lane.
 __device__ __forceinline__ void lds_copy4_global(const int32_t* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off"
                :
-               : "s"(lds), "v"(src)
+               : "s"(scalar(lds)), "v"(src)
                : "memory");
 }
 // All but the last N of this wave's copies have landed (they do in order).
@@ -392,9 +398,7 @@ __device__ __forceinline__ void stage_barrier() {
 
 // 16 bits of each wave, as one scalar.
 __device__ __forceinline__ uint64_t uniform64(const uint16_t* x) {
-  const uint64_t v = *(const uint64_t*)x;
-  return ((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) |
-         (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
+  return scalar(*(const uint64_t*)x);
 }
 
 // This wave's copies of a tile: K and V of keys 16w .. 16w + 15, whose pool rows (-1: zeros) lanes
@@ -481,7 +485,7 @@ struct Copier {
     const int key = key_of(i);
     int at;
     if (p.whole) {
-      const int e = __builtin_amdgcn_readfirstlane(s_ent[i & 127]);
+      const int e = scalar(s_ent[i & 127]);
       const int slot = key - div_by(key, p.block_div) * p.block_size;
       const int valid = e >= 0 && e < p.num_pool_blocks ? min(len - key, 16) : 0;
       const int64_t row = (int64_t)e * p.block_size + slot;
@@ -720,20 +724,20 @@ __device__ __forceinline__ u32x4 mark8(const Notes<kD>& row, int chunk, u32x4 v)
   return as_u32x4(h);
 }
 
-// x = cap_log2 * tanh(y), y = s * sm_scale / cap, in log2 units: tanh(y) = 1 - 2 / (1 + e^2y).
+// Capped scores in units of 2 cap: cap tanh(y) = cap - 2 cap / (1 + e^2y), and the softmax does not
+// change by a constant, so -1 / (1 + e^2y) will do (y = s * sm_scale / cap).
 __device__ __forceinline__ float capped(const Params& p, float s) {
-  const float e = fast_exp2(s * p.cap_exp);
-  return __builtin_fmaf(-2.f * p.cap_log2, __builtin_amdgcn_rcpf(1.f + e), p.cap_log2);
+  return -__builtin_amdgcn_rcpf(1.f + fast_exp2(s * p.cap_exp));
 }
-// The same for large caps, where the absolute error of that form would show: below 1/4 the series
-// (the next term is under 2e-8).
+// The same for large caps, where the absolute error of that form would show: tanh(y) / 2, below 1/4
+// from its series (the next term is under 2e-8).
 __device__ __forceinline__ float capped_series(const Params& p, float s) {
   const float y = s * (p.cap_exp * (0.5f / kLog2e)), z = y * y;
   float t = __builtin_fmaf(z, 62.f / 2835.f, -17.f / 315.f);
   t = __builtin_fmaf(z, t, 2.f / 15.f);
   t = __builtin_fmaf(z, t, -1.f / 3.f);
   t = __builtin_fmaf(z * y, t, y);
-  return __builtin_fabsf(y) < 0.25f ? p.cap_log2 * t : capped(p, s);
+  return __builtin_fabsf(y) < 0.25f ? 0.5f * t : 0.5f + capped(p, s);
 }
 
 // kSlices slices of 16 kT resident keys (k0 on) for this wave's rows.  s_pos, s_slope: of the wave's
@@ -778,7 +782,7 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
       for (int dt = 0; dt < kD / 16; ++dt) vf[dt] = vt_frag<kD, kT>(vs, c, dt);
     }
     if (kMod & kCap) {
-      const bool series = p.cap_log2 > kExpCap * kLog2e;
+      const bool series = p.scale_log2 > kExpCap * (2.f * kLog2e);
 #pragma unroll
       for (int j = 0; j < NB; ++j) {
         if (series) {
@@ -901,7 +905,7 @@ __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows
     int at = item - s.before;
     if (at == 0 && job.kvh == 0 && tid < 2) p.shares[2 * job.b + tid] = tid ? s.parts : s.before;
     if (at < rt.count * s.parts) {
-      part = __builtin_amdgcn_readfirstlane(whole_of(at, rt.count));
+      part = scalar(whole_of(at, rt.count));
       job.parts = s.parts;
       tile = rt.first + rt.count - 1 - (at - part * rt.count);
     } else {  // a row tile without tokens
@@ -913,14 +917,17 @@ __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows
     job.b = item - back * p.batch;
     tile = p.row_tiles - 1 - back;
   }
-  job.r0 = tile * tile_rows;
+  job.b = scalar(job.b);
+  job.parts = scalar(job.parts);
+  part = scalar(part);
+  job.r0 = scalar(tile) * tile_rows;
   job.row = row_of(p, job.b);
   int lo, hi;
   row_positions(p, job.row, job.r0, job.r0 + tile_rows - 1, lo, hi);
   job.span = span_of(p, job.row, lo, hi);
   const int size =
       job.parts == 1 ? job.span.n
-                     : __builtin_amdgcn_readfirstlane(parts_of(job.span.n, inverse(job.parts)));
+                     : scalar(parts_of(job.span.n, inverse(job.parts)));
   job.first = min(part * size, job.span.n);
   job.n = min(size, job.span.n - job.first);
   // a short list in few pieces: the other kernel reads no more
@@ -1528,9 +1535,8 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.head_dim = (int)head_dim;
   p.d_chunks = (int)(head_dim / 8);
   if (softcap > 0.f) {
-    p.scale_log2 = 1.f;
+    p.scale_log2 = softcap * (2.f * kLog2e);  // see capped()
     p.cap_exp = cap_arg * (2.f * kLog2e);
-    p.cap_log2 = softcap * kLog2e;
   } else {
     // scores are masked before they are scaled and -inf * 0 is NaN: a zero scale runs as unit
     // scale on a Q of zeros; a negative one on a negated Q
