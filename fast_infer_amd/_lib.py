@@ -223,6 +223,18 @@ def calls():
     return _calls
 
 
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def call_on(index: int, fn, *args):
+    """``fn(*args)`` with device `index` current: the default stream's handle is the same on every
+    device, and names the current one's."""
+    if _device() == index:
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
 def check(rc: int, what: str) -> None:
     if rc != FI_OK:
         msg = load().fi_last_error().decode(errors="replace")

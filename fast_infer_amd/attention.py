@@ -343,6 +343,8 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
             alibi_slopes = alibi_slopes.to(device=q.device, dtype=torch.float32)
         if not alibi_slopes.is_contiguous():
             alibi_slopes = alibi_slopes.contiguous()
+    if workspace is not None and (workspace.get_device() != dev or not workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous tensor on the same device as q")
     o = torch.empty_like(q)
     if batch == 0 or num_new == 0 or num_q_heads == 0:
         return o
@@ -359,7 +361,8 @@ def paged_chunk_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     ws_ptr = workspace.data_ptr() if need else None
     ws_bytes = workspace.numel() * workspace.element_size() if need else 0
-    rc = _lib.calls().fi_paged_chunk_attention_fwd(
+    rc = _lib.call_on(
+        dev, _lib.calls().fi_paged_chunk_attention_fwd,
         q_ptr, qs[0], qs[1], qs[2],
         k_cache.data_ptr(), v_cache.data_ptr(), num_blocks, block_size, num_kv_heads,
         block_table.data_ptr(), block_table.stride(0), bt_cols,

@@ -45,6 +45,9 @@ constexpr int64_t kWholeTokens = 512;
 // cap is an error of the logit, here 1e-4.
 constexpr float kExpCap = 500.f;
 
+constexpr float kMaxScale = 1e7f;  // scale or cap; the start of the running max stays finite in log2 units
+constexpr float kFlat = 1e-20f;
+
 constexpr int kCap = 1;   // kMod bits: capped scores,
 constexpr int kBias = 2;  // distance bias
 
@@ -1397,6 +1400,14 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
   return pl;
 }
 
+// |x| <= limit, false for NaN, by the bits: this file is compiled for NaN-free arithmetic.
+static bool within(float x, float limit) {
+  uint32_t a, b;
+  memcpy(&a, &x, 4);
+  memcpy(&b, &limit, 4);
+  return (a & 0x7fffffffu) <= b;
+}
+
 static bool sizes_ok(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads) {
   return batch >= 0 && chunk >= 0 && num_q_heads > 0 && num_kv_heads > 0 &&
          num_q_heads % num_kv_heads == 0;
@@ -1479,10 +1490,9 @@ extern "C" int fi_paged_chunk_attention_fwd(
     set_error("%s: window %lld must be positive, or 0 for none", fn, (long long)window);
     return FI_ERR_INVALID;
   }
-  const float cap_arg = softcap != 0.f ? sm_scale / softcap : 0.f;
-  if (!std::isfinite(sm_scale) || !std::isfinite(softcap) || softcap < 0.f || !std::isfinite(cap_arg)) {
-    set_error("%s: sm_scale %g and softcap %g must be finite, the cap positive (0 for none)", fn,
-              (double)sm_scale, (double)softcap);
+  if (!within(sm_scale, kMaxScale) || !within(softcap, kMaxScale) || softcap < 0.f) {
+    set_error("%s: sm_scale %g and softcap %g must be at most %g, the cap positive (0 for none)", fn,
+              (double)sm_scale, (double)softcap, (double)kMaxScale);
     return FI_ERR_INVALID;
   }
   if (batch == 0 || num_new == 0) return FI_OK;
@@ -1534,15 +1544,18 @@ extern "C" int fi_paged_chunk_attention_fwd(
   p.group_div = fast_div((uint32_t)p.group);
   p.head_dim = (int)head_dim;
   p.d_chunks = (int)(head_dim / 8);
-  if (softcap > 0.f) {
+  // Scores of a smaller scale or cap than kFlat differ by less than fp32 resolves in a weight: all
+  // zero, as with a scale of zero (scores are masked before they are scaled, and -inf * 0 is NaN).
+  const bool flat = std::fabs(sm_scale) < kFlat || (softcap > 0.f && softcap < kFlat);
+  const bool cap = softcap > 0.f && !flat;
+  if (cap) {
     p.scale_log2 = softcap * (2.f * kLog2e);  // see capped()
-    p.cap_exp = cap_arg * (2.f * kLog2e);
+    p.cap_exp = sm_scale / softcap * (2.f * kLog2e);
   } else {
-    // scores are masked before they are scaled and -inf * 0 is NaN: a zero scale runs as unit
-    // scale on a Q of zeros; a negative one on a negated Q
-    p.q_zero = sm_scale == 0.f;
+    // a zero scale runs as unit scale on a Q of zeros, a negative one on a negated Q
+    p.q_zero = flat;
     p.q_sign = sm_scale < 0.f ? 0x80008000u : 0u;
-    p.scale_log2 = p.q_zero ? kLog2e : std::fabs(sm_scale) * kLog2e;
+    p.scale_log2 = flat ? kLog2e : std::fabs(sm_scale) * kLog2e;
   }
   p.lazy_raw = kLazyLog2 / p.scale_log2;
   p.lazy_log2 = p.lazy_raw * p.scale_log2;
@@ -1581,7 +1594,7 @@ extern "C" int fi_paged_chunk_attention_fwd(
   if (pl.target) items = std::min(items + pl.parts() / num_kv_heads, items * std::max<int64_t>(most, 1));
   const dim3 grid((unsigned)(items * num_kv_heads));
   const hipStream_t st = (hipStream_t)stream;
-  const int mod = (softcap > 0.f ? kCap : 0) | (alibi_slopes ? kBias : 0);
+  const int mod = (cap ? kCap : 0) | (alibi_slopes ? kBias : 0);
   if (pl.width == 64)
     launch<64>(mod, pl, grid, st, p);
   else

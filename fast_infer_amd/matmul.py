@@ -247,9 +247,9 @@ def add_rms_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor,
         h = torch.empty_like(x, memory_format=torch.contiguous_format)
         h_stride, h_ptr = hidden, h.data_ptr()
     if rows:
-        rc = _lib.calls().fi_add_rmsnorm(x_ptr, x_stride, r_ptr, r_stride, rows, hidden,
-                                        weight.data_ptr(), float(eps), h_ptr, h_stride, out.data_ptr(),
-                                        hidden, _lib.tensor_stream(x))
+        rc = _lib.call_on(dev, _lib.calls().fi_add_rmsnorm, x_ptr, x_stride, r_ptr, r_stride, rows,
+                          hidden, weight.data_ptr(), float(eps), h_ptr, h_stride, out.data_ptr(),
+                          hidden, _lib.tensor_stream(x))
         _lib.check(rc, "add_rms_norm")
     return out, h
 

@@ -197,7 +197,8 @@ FI_API int fi_paged_attention_fwd_noalloc(const void* q, int64_t q_sb, int64_t q
  *   the row's length (the padding of a batch with fewer new tokens in some rows), and tokens that
  *   see no key, give zeros.  What the pool holds where a token does not look, infinities and
  *   NaN included, does not reach it.
- *   softcap     : 0, or cap > 0: x = cap * tanh(x / cap) for the scaled scores x = sm_scale * q.k
+ *   sm_scale    : any sign, at most 1e7 in size
+ *   softcap     : 0, or 0 < cap <= 1e7: x = cap * tanh(x / cap) for the scaled scores x = sm_scale * q.k
  *   alibi_slopes: NULL, or fp32[num_q_heads]: x -= slope * |pos - j|, after the cap
  *   window      : 0 for no window, else the number of positions a token sees up to its own
  *   prefix_lens : NULL, or int32[batch]: positions that every token of the row sees, before and

@@ -56,7 +56,8 @@ def _norm(**kw):
     (dict(cap=math.nan), _lib.FI_ERR_INVALID, b"softcap"),
     (dict(scale=math.nan), _lib.FI_ERR_INVALID, b"sm_scale"),
     (dict(scale=math.inf), _lib.FI_ERR_INVALID, b"sm_scale"),
-    (dict(cap=1e-40), _lib.FI_ERR_INVALID, b"softcap"),  # the scale over the cap overflows
+    (dict(cap=1.1e7), _lib.FI_ERR_INVALID, b"softcap"),
+    (dict(scale=-1.1e7), _lib.FI_ERR_INVALID, b"sm_scale"),
     (dict(batch=1, tokens=(1 << 22) + 1), _lib.FI_ERR_UNSUPPORTED, b"too large"),
     (dict(batch=1, blocks=1 << 26), _lib.FI_ERR_UNSUPPORTED, b"too large"),
     (dict(batch=1, new=1 << 27), _lib.FI_ERR_UNSUPPORTED, b"too large"),

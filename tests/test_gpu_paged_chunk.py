@@ -229,7 +229,7 @@ def test_infinite_values_that_are_seen(hip):
     assert ((out.double() - want[0]).abs() <= bound[0])[~touched].all()
 
 
-@pytest.mark.parametrize("scale", [0.0, -0.1, 2.0, 1e-6])
+@pytest.mark.parametrize("scale", [0.0, -0.1, 2.0, 1e-6, 1e-19, -1e-21, 1e-40])
 @pytest.mark.parametrize("opts", [{}, dict(softcap=10.0), dict(alibi=True), dict(softcap=3000.0, alibi=True)])
 def test_scales(hip, scale, opts):
     banner(f"chunk attention scale {scale} {opts}")
@@ -240,7 +240,7 @@ def test_scales(hip, scale, opts):
     _check(*_case(14, lens, 21, 6, 2, 64, 32), 32, lens, sm_scale=scale, window=70, **opts)
 
 
-@pytest.mark.parametrize("cap", [0.5, 500.0, 501.0, 1e5])
+@pytest.mark.parametrize("cap", [1e-40, 1e-19, 1e-3, 0.5, 500.0, 501.0, 1e5, 1e7])
 def test_caps(hip, cap):
     """Caps below the scores and far above them (where the plain form of tanh loses digits)."""
     banner(f"chunk attention cap {cap}")
@@ -409,6 +409,13 @@ def test_wrapper_refusals(hip):
             call(**kw)
     with pytest.raises(fi._lib.FastInferError):
         call(softcap=math.inf)
+    with pytest.raises(fi._lib.FastInferError):
+        fi.paged_chunk_attention(q, kc, vc, table, 64, 64, math.nan)
+    with pytest.raises(fi._lib.FastInferError):
+        fi.paged_chunk_attention(q, kc, vc, table, 64, -1)
+    for ws in (torch.empty(1 << 24, dtype=torch.uint8), torch.empty(1 << 24, 2, dtype=torch.uint8, device=DEV)[:, 0]):
+        with pytest.raises(ValueError):
+            call(workspace=ws)
     with pytest.raises(ValueError):
         fi.paged_chunk_attention(q, kc, vc, table, 32, 64)
     with pytest.raises(ValueError):
