@@ -1333,9 +1333,16 @@ constexpr int64_t kMaxWgs = (1 << 24) - 1;  // a launch takes fewer than 2^32 th
 struct Plan {
   bool narrow;
   int nb;
+  int64_t rows, row_lists;  // query rows of each (batch row, kv head), and how many of those
   int64_t row_tiles, wgs, target, target2, part_rows, width;
   int64_t tile_rows() const { return narrow ? 16 * nb : 64 * nb; }
   int64_t parts() const { return std::max(target, target2); }
+  void shape(int blocks) {
+    nb = blocks;
+    row_tiles = (rows + tile_rows() - 1) / tile_rows();
+    wgs = row_lists * row_tiles;
+    part_rows = std::min(rows, tile_rows());
+  }
   size_t bytes(int64_t batch) const {
     return (size_t)((parts() + wgs) * part_rows * (width + 2) + 2 * batch) * sizeof(float);
   }
@@ -1355,17 +1362,13 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
                  int64_t num_tokens, int64_t head_dim, int64_t window, bool lens,
                  bool may_cut) {
   constexpr int64_t kCus = 256;
-  const int64_t rows = chunk * (num_q_heads / num_kv_heads);
   Plan pl = {};
+  pl.rows = chunk * (num_q_heads / num_kv_heads);
+  pl.row_lists = batch * num_kv_heads;
   pl.width = head_dim <= 64 ? 64 : 128;
-  pl.narrow = rows <= 32;
-  auto shape = [&](int nb) {
-    pl.nb = nb;
-    pl.row_tiles = (rows + pl.tile_rows() - 1) / pl.tile_rows();
-    pl.wgs = batch * num_kv_heads * pl.row_tiles;
-  };
+  pl.narrow = pl.rows <= 32;
   if (pl.narrow) {
-    shape((int)((rows + 15) / 16));
+    pl.shape((int)((pl.rows + 15) / 16));
     const int64_t slots = pl.width == 64 ? 4 * kCus : 2 * kCus;
     pl.target = may_cut && pl.wgs < slots && num_tokens > kWholeTokens ? slots : 0;
   } else {
@@ -1376,7 +1379,7 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
     int nb = 0;
     bool cut = false;
     for (int i = 1; i <= 3; ++i) {
-      shape(i);
+      pl.shape(i);
       const int64_t span = window + pl.tile_rows() / (num_q_heads / num_kv_heads) + kKTile;
       const double n = (double)((std::min(num_tokens, span) + kKTile - 1) / kKTile);
       const double alone = wide * kAlone[i - 1], shared = wide * kShared[i - 1];
@@ -1392,11 +1395,10 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
         if (pieces < best) best = pieces, nb = i, cut = true;
       }
     }
-    shape(nb);
+    pl.shape(nb);
     pl.target = cut ? 2 * kCus : 0;
     pl.target2 = cut && ragged ? 4 * kCus : 0;
   }
-  pl.part_rows = pl.target ? std::min<int64_t>(rows, pl.tile_rows()) : 0;
   return pl;
 }
 
@@ -1448,12 +1450,18 @@ extern "C" size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t
       max_num_tokens <= 0 || max_num_tokens > kMaxTokens || !fi::head_dim_ok(head_dim) ||
       batch > 0x7fffffff || num_new > 0x7fffffff / num_q_heads)
     return 0;
-  // whether the call will have lengths of its own, or a window, is not known here: the most of these
+  // whether the call will have lengths of its own, or a window (which may choose other row blocks),
+  // is not known here: the most of these
   size_t bytes = 0;
   for (const bool lens : {false, true}) {
-    const Plan pl =
+    Plan pl =
         plan(batch, num_new, num_q_heads, num_kv_heads, max_num_tokens, head_dim, kNoWindow, lens, true);
-    if (pl.target) bytes = std::max(bytes, pl.bytes(batch));
+    if (!pl.target) continue;
+    bytes = std::max(bytes, pl.bytes(batch));
+    for (int nb = 1; nb <= 3 && !pl.narrow; ++nb) {
+      pl.shape(nb);
+      if (pl.wgs < pl.target) bytes = std::max(bytes, pl.bytes(batch));
+    }
   }
   return bytes;
 }
@@ -1482,8 +1490,8 @@ extern "C" int fi_paged_chunk_attention_fwd(
               (long long)num_tokens);
     return FI_ERR_INVALID;
   }
-  if (block_size <= 0) {
-    set_error("%s: block_size %lld must be positive", fn, (long long)block_size);
+  if (block_size <= 0 || block_size > 0x7fffffff) {
+    set_error("%s: block_size %lld must be positive, below 2^31", fn, (long long)block_size);
     return FI_ERR_INVALID;
   }
   if (window < 0) {

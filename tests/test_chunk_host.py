@@ -50,6 +50,7 @@ def _norm(**kw):
     (dict(blocks=-1), _lib.FI_ERR_INVALID, b"invalid sizes"),
     (dict(max_blocks=-1), _lib.FI_ERR_INVALID, b"invalid sizes"),
     (dict(bs=0), _lib.FI_ERR_INVALID, b"block_size 0"),
+    (dict(batch=1, bs=1 << 32, blocks=0), _lib.FI_ERR_INVALID, b"block_size 4294967296"),
     (dict(window=-5), _lib.FI_ERR_INVALID, b"window -5"),
     (dict(cap=-1.0), _lib.FI_ERR_INVALID, b"softcap -1"),
     (dict(cap=math.inf), _lib.FI_ERR_INVALID, b"softcap inf"),
@@ -93,6 +94,9 @@ def test_chunk_workspace_size(lib):
     for bad in ((0, 4, 24, 8, 4096, 128), (1, 0, 24, 8, 4096, 128), (1, 4, 20, 8, 4096, 128),
                 (1, 4, 24, 8, 0, 128), (1, 4, 24, 8, 4096, 60), (1, 4, 24, 8, (1 << 22) + 1, 128)):
         assert size(*bad) == 0
+    # a window may choose other row blocks: 106 rows of 16 keys or more a wave, parts of one round
+    # of 512 workgroups, 128 columns, a maximum and a sum
+    assert size(1, 106, 1, 1, 17117, 128) >= (512 + 1) * 106 * 130 * 4 + 8
     # bounded whatever the sizes
     rng = random.Random(3)
     for _ in range(200):
