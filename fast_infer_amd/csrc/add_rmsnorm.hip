@@ -4,8 +4,9 @@
 //   out = fp16((h * r) * weight),  r = rsqrt(sum(h^2) / hidden + eps), in fp32 from the rounded h
 //
 // i.e. an addition followed by rms_norm, in one pass: each element of x and residual is read
-// once, h and out are written once (8 bytes an element; the two calls move 12).  Bound by
-// memory, and by latency for few rows.  A row is held in registers between the sum of squares
+// once, h and out are written once (8 bytes an element; the two calls move 10).  Bound by
+// memory (16384 x 5120, 671 MB: 104 us, 6.4 TB/s), and by latency for few rows (1 x 4096 1.9 us, 777 x
+// 2560 4.5 us from the cache).  A row is held in registers between the sum of squares
 // and the scaling; rows of more than kMaxHeld elements are read back from h.
 #include <algorithm>
 
@@ -22,7 +23,7 @@ constexpr int kMaxHeld = kThreads * 8 * kMaxParts;  // 8192
 // 20 -> 18, 30000 x 1024 40 -> 38.
 constexpr int kNarrow = 1024;
 // Bytes moved from which the non-temporal policy pays, beyond the last-level cache: 16384 x 5120
-// 116 -> 110 us (6.1 TB/s); 30000 x 1024 (246 MB) 40 against 42.
+// 116 -> 110 us a call; 30000 x 1024 (246 MB) 40 against 42.
 constexpr int64_t kCached = (int64_t)400 << 20;
 
 struct Params {

@@ -10,17 +10,22 @@
 //             j < prefix, or pos - window < j <= pos
 //
 // Layout for MI355X:
-//   * The query rows of one kv head are the pairs (token, head of the group), token-major, and a
-//     workgroup takes 64 * NB consecutive ones, whatever the group size: 16 * NB per wave, one
-//     row per MFMA column.  Each 64-key K/V tile staged in LDS serves all of them.
+//   * The query rows of one kv head are the pairs (token, head of the group), token-major, one row
+//     per MFMA column, so that any group size fills the columns.  Up to 32 rows (single tokens,
+//     drafted ones) are bound by the stream of K and V: narrow_kernel, whose waves share the rows
+//     and split the keys.  More rows are bound by the matrix cores and the softmax beside them:
+//     chunk_kernel, whose waves share the key tiles and have 16 to 48 rows each.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: the lane that holds a query
 //     column keeps its scores, P and O; the softmax (online, fp32, base 2) needs no shuffles.
-//   * Tiles are copied global -> LDS without registers, two stages.  Every lane carries the
-//     64-bit address of its own piece of a key's row, looked up in the block table one tile
-//     ahead, so that any block size and any pool size take the same path; keys at or past the
-//     row's length, or behind an invalid table entry, are read from a page of zeros.
-//   * Few query rows: the row tile's list of key tiles is cut into parts, by its own true
-//     length, on the device; the parts' unnormalised results are added by a second kernel.
+//   * 64-key tiles are copied global -> LDS without registers, the next one while one is used; so
+//     are the block table's entries.  Keys at or past the row's length, or behind an invalid
+//     entry, are copied from a row of zeros, and never read.
+//   * The tiles that need a mask (the diagonal, the ends of the window and of the prefix) come first, in
+//     a loop of their own: the others run without any (233 -> 92 us for 512 tokens at 8192).
+//   * Where the row tiles alone do not fill the device their lists of key tiles are cut into parts, by
+//     the rows' own lengths, on the device; a second kernel adds the parts.
+// Measured (24 query heads on 8 kv heads, 128 wide, MI355X): 2 x 2048 tokens, of 16384, 0.72-0.73 ms, 1.06
+// PFLOP/s; 512 tokens at 8192 73 us, 0.69; 24 rows of 5 drafted tokens (300 to 4096 keys) 45 us, 4.5 TB/s.
 #include <algorithm>
 #include <climits>
 #include <cmath>
@@ -46,7 +51,7 @@ constexpr int64_t kWholeTokens = 512;
 constexpr float kExpCap = 500.f;
 
 constexpr float kMaxScale = 1e7f;  // scale or cap; the start of the running max stays finite in log2 units
-constexpr float kFlat = 1e-20f;
+constexpr float kFlat = 1e-20f;    // scale or cap below which every score counts as zero
 
 constexpr int kCap = 1;   // kMod bits: capped scores,
 constexpr int kBias = 2;  // distance bias
@@ -937,7 +942,11 @@ __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows
   return job.parts == 1 || job.n > 0;
 }
 
-// Many rows: the waves share the tiles, each with rows of its own.
+// Many rows: the waves share the tiles, each with 16 NB rows of its own, so that a tile read once
+// from memory and a fragment read once from LDS serve many.  Bound by the matrix cores and the
+// softmax, which the two workgroups of a CU overlap in part: a tile of three blocks takes 2780
+// cycles, 1632 of them MFMA (16384 keys; the two together 1.06 PFLOP/s, the library's largest fp16
+// products 1.2 to 1.45).  A cap adds an exp2 and a reciprocal a score, about a third.
 template <int NB, int kD, int kMod>
 __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
   typedef Tile<kD> T;
@@ -1084,8 +1093,10 @@ __global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
 
 // Few rows (at most 16 NB): every wave has all of them and takes 16 keys of each tile, those that it
 // copies itself, so the waves run without barriers, each waiting for its own copies only, and
-// are added up through LDS at the end.  Bound by the stream of K and V: with the rows of one
-// wave and shared tiles, 2.9 TB/s.
+// are added up through LDS at the end.  Bound by the stream of K and V, which a kv head reads in
+// slices of 256 bytes (5.2 to 5.8 TB/s for such a read alone): 24 rows of 5 drafted tokens, 203 MB, 39 us
+// of which about 6 pass before the first tile (the work list, the table, the first copies), 32 single
+// capped tokens, 335 MB, 62; 2.9 TB/s when the waves shared the tiles as in chunk_kernel.
 template <int NB, int kD, int kMod>
 __global__ __launch_bounds__(kThreads, kD == 64 ? 4 : 2) void narrow_kernel(Params p) {
   typedef Tile<kD> T;
@@ -1239,7 +1250,8 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 4 : 2) void narrow_kernel(Para
 // columns a lane; grid (rows of a batch row, batch).  Batch rows that were not cut, and row tiles
 // without a token, were written by the kernels above.  All loads of a few parts are issued at once;
 // with kSpread (few rows in many parts) the workgroup has one row and each kD / 4 lanes every
-// 1024 / kD-th part, added up through LDS.
+// 1024 / kD-th part, added up through LDS.  4.0 to 4.7 us for few rows, most of it the launch; 512
+// tokens in 8 parts, 50 MB, 10.8 us (4.7 TB/s).
 constexpr int kMergeThreads = 256;
 struct Sum {
   float m = kNegBig, l = 0.f;

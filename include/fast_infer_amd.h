@@ -205,7 +205,7 @@ FI_API int fi_paged_attention_fwd_noalloc(const void* q, int64_t q_sb, int64_t q
  *                 behind it (a prefix mask; with a window, tokens that stay visible)
  *   workspace   : fi_paged_chunk_attention_workspace_size(batch, num_new, num_q_heads,
  *                 num_kv_heads, num_tokens, head_dim) bytes, 16-byte aligned; it needs no
- * *   initialisation.  With less (or NULL) the context is not cut into parts: slower.
+ *                 initialisation.  With less (or NULL) the context is not cut into parts: slower.
  *                 Calls that overlap in time must not share it.
  */
 FI_API size_t fi_paged_chunk_attention_workspace_size(int64_t batch, int64_t num_new,

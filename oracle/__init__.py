@@ -20,6 +20,8 @@ Contents (each function cites the reference file:line it restates):
 * ``int4`` — numpy restatement of the INT4 weight format: quantize (loader.py:9-41),
   unpack / dequantize (matmul.py:309-326), and the float64 product with its error bound.
 * ``rmsnorm`` — RMSNorm (kernels/rms_norm.py:8-43) in float64 and its fp16 error bound.
+* ``chunk`` — attention of new tokens over the paged pool with its score options, and RMSNorm
+  with the residual's addition, in float64 with their error bounds (no counterpart in the reference).
 * ``ref_algo.c`` (+ ``native``) — the same tile algorithms in C with OpenMP, used
   as the CPU baseline ("port").
 
