@@ -948,7 +948,7 @@ __device__ __forceinline__ bool find_job(const Params& p, int tid, int tile_rows
 // cycles, 1632 of them MFMA (16384 keys; the two together 1.06 PFLOP/s, the library's largest fp16
 // products 1.2 to 1.45).  A cap adds an exp2 and a reciprocal a score, about a third.
 template <int NB, int kD, int kMod>
-__global__ __launch_bounds__(kThreads, 2) void chunk_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void chunk_kernel(Params p) {
   typedef Tile<kD> T;
   constexpr int kRowsPerWave = 16 * NB;
   constexpr int kRows = kWaves * kRowsPerWave;
@@ -1368,8 +1368,13 @@ struct Plan {
 // 1.1, 1.5 for 1, 2, 3 blocks (128 wide; chunks of 512 tokens at 8192, 2 x 1000 at 5000, 2 x 2048
 // at 16384).  A call costs 6 us besides, one that is cut 6 more, and a round of parts 6 us per
 // block for results written and read.  Rows of one call that have their own lengths are taken to
-// have two thirds of the bound on average, the longest the whole.  Against three blocks always: 4 x 128
-// tokens at 300 29 -> 14 us, a prompt of 512 25 -> 16, 2 x 1000 at 5000 214 -> 175.
+// have two thirds of the bound on average, the longest the whole; the row tiles of one row the mean
+// of its first and last token's keys (a prompt of 2000 tokens 75 -> 49 us, of 4096 152 -> 134, against all
+// the last token's).  The 64-wide form takes 0.6 of that time, and has room for three workgroups per CU
+// (two: 2 x 1000 tokens at 8000 102 us against 92, 1500 at 20000 173 against 149).  The choice is
+// within 5% of the best of the six but for single cases (8 x 300 tokens at 3000: 85 against 77).
+// Against three blocks, uncut: 4 x 128 tokens at 300 20 -> 13 us, a prompt of 512 25 -> 15.5, 2 x
+// 1000 at 5000 201 -> 169.
 static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_kv_heads,
                  int64_t num_tokens, int64_t head_dim, int64_t window, bool lens,
                  bool may_cut) {
@@ -1385,6 +1390,8 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
     pl.target = may_cut && pl.wgs < slots && num_tokens > kWholeTokens ? slots : 0;
   } else {
     static constexpr double kAlone[3] = {1.17, 1.74, 2.08}, kShared[3] = {0.72, 1.1, 1.5};
+    const int64_t per_slot = pl.width == 64 ? 3 : 2;  // workgroups of a CU
+    const int64_t slots = per_slot * kCus;
     const double wide = pl.width == 64 ? 0.6 : 1.0;
     const bool ragged = lens && batch > 1;
     double best = 0;
@@ -1394,22 +1401,25 @@ static Plan plan(int64_t batch, int64_t chunk, int64_t num_q_heads, int64_t num_
       pl.shape(i);
       const int64_t span = window + pl.tile_rows() / (num_q_heads / num_kv_heads) + kKTile;
       const double n = (double)((std::min(num_tokens, span) + kKTile - 1) / kKTile);
+      // the first tokens of the chunk see fewer keys
+      const double mean = num_tokens <= span ? n - (double)std::min(chunk, num_tokens) / (2 * kKTile) : n;
       const double alone = wide * kAlone[i - 1], shared = wide * kShared[i - 1];
       const int64_t per_cu = (pl.wgs + kCus - 1) / kCus;
-      const double whole = 6 + n * (per_cu == 1 ? alone : (double)per_cu * shared);
+      const double whole = 6 + (per_cu == 1 ? n * alone : std::max(n * alone, (double)per_cu * mean * shared));
       if (nb == 0 || whole < best) best = whole, nb = i, cut = false;
-      const int64_t parts = std::min<int64_t>(2 * kCus / pl.wgs, (int64_t)n / kMinPart);
-      if (may_cut && pl.wgs < 2 * kCus && (parts >= 2 || (ragged && n > 2 * kMinPart))) {
-        const double round = std::min(1.0, (double)(pl.wgs * std::max<int64_t>(parts, 1)) / (2 * kCus));
+      const int64_t parts = std::min<int64_t>(slots / pl.wgs, (int64_t)n / kMinPart);
+      if (may_cut && pl.wgs < slots && (parts >= 2 || (ragged && n > 2 * kMinPart))) {
+        const double round = std::min(1.0, (double)(pl.wgs * std::max<int64_t>(parts, 1)) / slots);
         double chain = ceil(n / (double)std::max<int64_t>(parts, 1));
-        if (ragged) chain = (0.65 + 0.7 / (double)batch) * n * (double)pl.wgs / (2 * kCus);
-        const double pieces = 12 + chain * (round <= 0.5 && !ragged ? alone : 2 * shared) + 6 * wide * i * (ragged ? 1.0 : round);
+        if (ragged) chain = (0.65 + 0.7 / (double)batch) * n * (double)pl.wgs / slots;
+        const double step = round * per_slot <= 1 && !ragged ? alone : per_slot * shared;
+        const double pieces = 12 + chain * step + 6 * wide * i * (ragged ? 1.0 : round);
         if (pieces < best) best = pieces, nb = i, cut = true;
       }
     }
     pl.shape(nb);
-    pl.target = cut ? 2 * kCus : 0;
-    pl.target2 = cut && ragged ? 4 * kCus : 0;
+    pl.target = cut ? slots : 0;
+    pl.target2 = cut && ragged ? 2 * slots : 0;
   }
   return pl;
 }
