@@ -525,10 +525,21 @@ struct Copier {
   }
 };
 
-// A slice of 16 kT keys (kT = 2 or 1) is what one step of the softmax covers.  P and V^T fragments
-// hold 4 kT keys a lane: with kT = 2 keys 4g + j and 16 + 4g + j (j = 0..3) in slots j and 4 + j.
+// A slice of 16 kT keys (kT = 4, 2 or 1) is what one step of the softmax covers.  P and V^T fragments
+// hold 4 kT keys a lane: keys 16 t + 4g + j (j = 0..3) in slots 4 t + j.
+typedef _Float16 half16 __attribute__((ext_vector_type(16)));
 template <int kT>
 struct Slice;
+template <>
+struct Slice<4> {
+  typedef half16 frag;
+  static __device__ __forceinline__ floatx4 mfma(half16 a, half16 b, floatx4 c) {
+    return mfma16x16x32(__builtin_shufflevector(a, a, 8, 9, 10, 11, 12, 13, 14, 15),
+                        __builtin_shufflevector(b, b, 8, 9, 10, 11, 12, 13, 14, 15),
+                        mfma16x16x32(__builtin_shufflevector(a, a, 0, 1, 2, 3, 4, 5, 6, 7),
+                                     __builtin_shufflevector(b, b, 0, 1, 2, 3, 4, 5, 6, 7), c));
+  }
+};
 template <>
 struct Slice<2> {
   typedef half8 frag;
@@ -560,14 +571,15 @@ template <int kD, int kT>
 __device__ __forceinline__ typename Slice<kT>::frag vt_frag(uint32_t vs, int c, int dt) {
   typedef short s4 __attribute__((ext_vector_type(4)));
   typedef s4 __attribute__((address_space(3))) * lds_s4;
-  const uint32_t at = (vs ^ (dt << 5)) + 16 * kT * c * Tile<kD>::kRow;
-  const half4 a = __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at));
   if constexpr (kT == 1) {
-    return a;
+    const uint32_t at = (vs ^ (dt << 5)) + 16 * c * Tile<kD>::kRow;
+    return __builtin_bit_cast(half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)at));
+  } else if constexpr (kT == 2) {
+    return __builtin_shufflevector(vt_frag<kD, 1>(vs, 2 * c, dt), vt_frag<kD, 1>(vs, 2 * c + 1, dt), 0, 1, 2, 3, 4,
+                                   5, 6, 7);
   } else {
-    const half4 b = __builtin_bit_cast(
-        half4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(at + 16 * Tile<kD>::kRow)));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    return __builtin_shufflevector(vt_frag<kD, 2>(vs, 2 * c, dt), vt_frag<kD, 2>(vs, 2 * c + 1, dt), 0, 1, 2, 3, 4,
+                                   5, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15);
   }
 }
 
@@ -811,17 +823,17 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
       for (int j = 0; j < NB; ++j) {
         // without branches: as conditions they took three times a full tile's time
         const int back = s_pos[16 * j + col] - key0, ahead = prefix - key0;
-        const uint32_t here = (uint32_t)(keys >> (16 * kT * c)) >> (4 * g);
+        const uint64_t here = keys >> (16 * kT * c) >> (4 * g);
 #pragma unroll
         for (int e = 0; e < kE; ++e) {
           const int at = 16 * (e >> 2) + (e & 3);
           const bool see = (((uint32_t)(back - at) < (uint32_t)p.window) | (ahead > at)) &
-                           (((here >> at) & 1) != 0);
+                           (((uint32_t)(here >> (at & 32)) >> (at & 31) & 1) != 0);
           s[j][e >> 2][e & 3] = see ? s[j][e >> 2][e & 3] : -__builtin_inff();
         }
       }
     } else if (keys != kAll) {  // missing table entries
-      const uint32_t here = (uint32_t)(keys >> (16 * kT * c)) >> (4 * g);
+      const uint64_t here = keys >> (16 * kT * c) >> (4 * g);
 #pragma unroll
       for (int j = 0; j < NB; ++j)
 #pragma unroll
@@ -835,8 +847,9 @@ __device__ __forceinline__ void consume(const Params& p, uint32_t ks, uint32_t v
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
       lmax[j] = fmaxf(fmaxf(s[j][0][0], s[j][0][1]), fmaxf(s[j][0][2], s[j][0][3]));
-      if constexpr (kT == 2)
-        lmax[j] = fmaxf(fmaxf(fmaxf(s[j][1][0], s[j][1][1]), fmaxf(s[j][1][2], s[j][1][3])), lmax[j]);
+#pragma unroll
+      for (int t = 1; t < kT; ++t)
+        lmax[j] = fmaxf(fmaxf(fmaxf(s[j][t][0], s[j][t][1]), fmaxf(s[j][t][2], s[j][t][3])), lmax[j]);
       move |= lmax[j] > t_run[j];
     }
     if (__builtin_amdgcn_ballot_w64(move)) {
@@ -952,6 +965,10 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void chunk_kernel(Param
   typedef Tile<kD> T;
   constexpr int kRowsPerWave = 16 * NB;
   constexpr int kRows = kWaves * kRowsPerWave;
+  // Two slices a tile; one row block alone waits for each step in turn and takes the tile in one (777
+  // tokens of 3 rows, 64 wide, 23 -> 20.7 us, a prompt of 2000 51 -> 49; with a cap, whose steps wait less, 27
+  // -> 39 for 250 tokens at 1500).
+  constexpr int kT = NB == 1 && !(kMod & kCap) ? 4 : 2;
   __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
   __shared__ int s_pos[kRows];  // position of each query row, -1 for rows without a token
   __shared__ float s_slope[kMod & kBias ? kRows : 1];  // its distance bias in score units
@@ -1029,14 +1046,14 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void chunk_kernel(Param
       noted = true;
     }
     if (wlo <= whi && (k0 < row.prefix || (k0 <= whi && k0 + kKTile > wlo - p.window + 1)))
-      consume<NB, kD, kMod, 2, 2, true>(p, ks + at, vs + at, k0, keys, row.prefix, w_pos, w_slope, col, g, qf,
+      consume<NB, kD, kMod, kT, 4 / kT, true>(p, ks + at, vs + at, k0, keys, row.prefix, w_pos, w_slope, col, g, qf,
                                         t_run, acc);
     stage_barrier();
   }
   for (; i < n; ++i) {
     const uint64_t keys = copy_next(i);
     if (wlo <= whi)
-      consume<NB, kD, kMod, 2, 2, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
+      consume<NB, kD, kMod, kT, 4 / kT, false>(p, ks + (i & 1) * T::kStage, vs + (i & 1) * T::kStage,
                                          span.tile(first + i) * kKTile, keys, row.prefix, w_pos, w_slope,
                                          col, g, qf, t_run, acc);
     stage_barrier();
