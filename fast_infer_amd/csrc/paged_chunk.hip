@@ -965,10 +965,12 @@ __global__ __launch_bounds__(kThreads, kD == 64 ? 3 : 2) void chunk_kernel(Param
   typedef Tile<kD> T;
   constexpr int kRowsPerWave = 16 * NB;
   constexpr int kRows = kWaves * kRowsPerWave;
-  // Two slices a tile; one row block alone waits for each step in turn and takes the tile in one (777
-  // tokens of 3 rows, 64 wide, 23 -> 20.7 us, a prompt of 2000 51 -> 49; with a cap, whose steps wait less, 27
-  // -> 39 for 250 tokens at 1500).
-  constexpr int kT = NB == 1 && !(kMod & kCap) ? 4 : 2;
+  // Two slices a tile, or one where the registers allow it, whose steps wait for one another half as
+  // often: one row block, 777 tokens of 3 rows, 64 wide, 23 -> 20.7 us, a prompt of 2000 51 -> 49; two blocks,
+  // 128 wide, 4096 tokens 129 -> 122, 4 x 1000 at 5000 with biases 349 -> 324 (64 wide 60.4 -> 61.6).  With a
+  // cap 27 -> 39 for 250 tokens at 1500 and 68 -> 77 for 2 x 1000.
+  constexpr bool kOne = (NB == 1 || (NB == 2 && kD == 128)) && !(kMod & kCap);
+  constexpr int kT = kOne ? 4 : 2;
   __shared__ __attribute__((aligned(16))) char stages[2 * T::kStage];
   __shared__ int s_pos[kRows];  // position of each query row, -1 for rows without a token
   __shared__ float s_slope[kMod & kBias ? kRows : 1];  // its distance bias in score units
