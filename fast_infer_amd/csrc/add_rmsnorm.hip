@@ -5,7 +5,7 @@
 //
 // i.e. an addition followed by rms_norm, in one pass: each element of x and residual is read
 // once, h and out are written once (8 bytes an element; the two calls move 10).  Bound by
-// memory (16384 x 5120, 671 MB: 104 us, 6.4 TB/s), and by latency for few rows (1 x 4096 1.9 us, 777 x
+// memory (16384 x 5120, 671 MB: 104 to 108 us, 6.2 to 6.4 TB/s), and by latency for few rows (1 x 4096 1.8 us, 777 x
 // 2560 4.5 us from the cache).  A row is held in registers between the sum of squares
 // and the scaling; rows of more than kMaxHeld elements are read back from h.
 #include <algorithm>

@@ -24,7 +24,7 @@
 //     a loop of their own: the others run without any (233 -> 92 us for 512 tokens at 8192).
 //   * Where the row tiles alone do not fill the device their lists of key tiles are cut into parts, by
 //     the rows' own lengths, on the device; a second kernel adds the parts.
-// Measured (24 query heads on 8 kv heads, 128 wide, MI355X): 2 x 2048 tokens, of 16384, 0.72-0.73 ms, 1.06
+// Measured (24 query heads on 8 kv heads, 128 wide, MI355X): 2 x 2048 tokens, of 16384, 0.72-0.74 ms, 1.06
 // PFLOP/s; 512 tokens at 8192 73 us, 0.69; 24 rows of 5 drafted tokens (300 to 4096 keys) 45 us, 4.5 TB/s.
 #include <algorithm>
 #include <climits>
