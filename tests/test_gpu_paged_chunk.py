@@ -490,3 +490,60 @@ def test_long_parts(hip, bs, new):
     assert rc == 0
     ok, msg = OC.is_close(o, exact, bound)
     assert ok, msg
+
+
+# (batch, kv heads, group, new tokens, longest row, head_dim, block size): row tiles that fill the
+# device, with two and three row blocks a wave, and fewer of them over longer rows, cut into parts
+MANY_ROWS = [(4, 8, 8, 193, 242, 128, 16), (4, 8, 8, 260, 367, 128, 64), (4, 8, 8, 193, 220, 64, 24),
+             (4, 8, 8, 274, 379, 64, 16), (2, 8, 1, 582, 3619, 128, 64), (4, 8, 3, 174, 3747, 128, 32),
+             (1, 4, 6, 534, 3085, 120, 48), (2, 8, 2, 291, 3600, 64, 16), (4, 8, 1, 524, 3737, 64, 40)]
+
+
+@pytest.mark.parametrize("opts", [{}, {"softcap": 20.0}, {"alibi": 1, "prefix": 150},
+                                  {"softcap": 900.0, "alibi": 1, "window": 100, "prefix": 70}],
+                         ids=["plain", "cap", "bias", "all"])
+@pytest.mark.parametrize("shape", MANY_ROWS, ids=lambda s: "x".join(map(str, s)))
+def test_many_query_rows(hip, shape, opts):
+    """Chunks of many query rows, the rows of the batch at different lengths and padded but for one."""
+    banner(f"chunk attention many rows {shape} {opts}")
+    batch, hkv, group, new, longest, d, bs = shape
+    lens = [longest - 37 * b * (longest // 150) for b in range(batch)]
+    starts = [n - new + 11 * b for b, n in enumerate(lens)]
+    kw = dict(opts)
+    if kw.pop("alibi", None):
+        kw["alibi_slopes"] = _slopes(group * hkv)
+    if "prefix" in kw:
+        kw["prefix"] = [kw["prefix"] >> b for b in range(batch)]
+    q, kc, vc, table = _case(27, lens, new, group * hkv, hkv, d, bs, spread=3.0 if "softcap" in kw else 1.0)
+    out = _check(q, kc, vc, table, bs, lens, starts, **kw)
+    for b in range(1, batch):
+        assert not out[b, new - 11 * b:].any()
+
+
+@pytest.mark.parametrize("shape", MANY_ROWS[1:4] + MANY_ROWS[5:8], ids=lambda s: "x".join(map(str, s)))
+def test_infinite_values_of_many_query_rows(hip, shape):
+    """Infinite values of V at the chunk's own positions reach the tokens that see them and no others."""
+    banner(f"chunk attention infinities many rows {shape}")
+    import fast_infer_amd as fi
+
+    batch, hkv, group, new, longest, d, bs = shape
+    lens = [longest - 20 * b for b in range(batch)]
+    starts = [n - new + b for b, n in enumerate(lens)]
+    q, kc, vc, table = _case(28, lens, new, group * hkv, hkv, d, bs)
+    want, bound = OC.chunk_attention(q, kc, vc, table, bs, lens, starts, window=90)
+    spots = [(b, starts[b] + t, (3 * t) % hkv, (17 * t) % d) for b in range(batch) for t in (5, new // 2, new - 9)]
+    # (the third and fourth rows of the shorter chunks begin before position 0: their first spot is an
+    # index from the table's end, of a slot that may be another row's.  So what each row holds is read back.)
+    for b, pos, h, c in spots:
+        vc[table[b, pos // bs].long(), pos % bs, h, c] = math.inf
+    for b in range(batch):
+        pos = torch.arange(lens[b], device=DEV)
+        rows = vc[table[b, pos // bs].long(), pos % bs]
+        for at, h, c in torch.isinf(rows).nonzero().tolist():
+            t0, t1 = max(at - starts[b], -starts[b], 0), min(at - starts[b] + 90, lens[b] - starts[b])
+            want[b, t0:max(t1, t0), group * h:group * h + group, c] = math.inf
+    out = fi.paged_chunk_attention(q, kc, vc, table, bs, longest, start_positions=_i32(starts),
+                                   context_lens=_i32(lens), window=90)
+    finite = torch.isfinite(want)
+    assert torch.equal(out.double()[~finite], want[~finite])
+    assert ((out.double() - want).abs() <= bound)[finite].all()
